@@ -108,10 +108,10 @@ def _lengths(case):
 
 
 def _exponent(amax):
-    """The smallest e with amax <= 448 * 2^e, at least -64; 0 for a block of zeros."""
+    """The smallest e with amax <= 448 * 2^e, at least -64."""
     m, x = torch.frexp(amax)
     e = torch.where(m <= 0.875, x - 9, x - 8).clamp_min(-64)
-    return torch.where(amax > 0, e, torch.zeros_like(e)).to(torch.int32)
+    return torch.where(amax > 0, e, torch.full_like(e, -64)).to(torch.int32)
 
 
 def _pow2(e):
@@ -442,7 +442,7 @@ def _smallest_exponent(a):
     e = -64
     while a > 448.0 * 2.0 ** e:
         e += 1
-    return e if a > 0 else 0
+    return e
 
 
 class _Exact8:
@@ -541,7 +541,7 @@ def _exact_rows(s):
             e = torch.ceil(torch.log2(top / 448.0)).clamp_min(-64)
             e = torch.where(448.0 * torch.exp2(e - 1) >= top, e - 1, e).clamp_min(-64)
             e = torch.where(top > 448.0 * torch.exp2(e), e + 1, e)
-            e = torch.where(top > 0, e, torch.zeros_like(e))
+            e = torch.where(top > 0, e, torch.full_like(e, -64.0))
             if first % BLOCK:
                 was = float(s["scales"][page[0], slot[0] // BLOCK, k])
                 e[0] = max(float(e[0]), was)
