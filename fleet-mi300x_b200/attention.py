@@ -30,7 +30,7 @@ import numpy as np
 import torch
 
 from . import native
-from .cache import PagedLatentCache
+from .cache import PagedLatentCache, PagedLatentCache8
 from .config import ModelConfig, rope_tables
 
 
@@ -65,6 +65,11 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _scales_ptr(cache: PagedLatentCache) -> int | None:
+    """The exponents of an 8-bit cache, None for a bf16 one."""
+    return cache.scales.data_ptr() if isinstance(cache, PagedLatentCache8) else None
+
+
 class MlaDecodeAttention:
     """One layer's attention task over a PagedLatentCache.
 
@@ -75,8 +80,12 @@ class MlaDecodeAttention:
 
     def __init__(self, cfg: ModelConfig, w: LayerWeights, rope_cos: torch.Tensor, rope_sin: torch.Tensor,
                  *, num_ctas: int = 0, check_kernel: bool = False, kernel: str = "mma", qc_hilo: bool = False,
-                 p_hilo: bool = False):
-        """qc_hilo / p_hilo (default kernel only): keep the absorbed query, and the
+                 p_hilo: bool = False, window: int = 0, sinks: int = 0):
+        """Every call takes either cache class; on a PagedLatentCache8 the 8-bit split-KV
+        kernel runs (check_kernel, kernel="tcgen05" and the hi/lo forms are the bf16 cache's).
+        window > 0: a query sees the last `window` rows of its request, its own among them, and the first
+        `sinks` rows; pages without a visible row are not read (and their block-table entries
+        need not be valid). qc_hilo / p_hilo (default kernel only): keep the absorbed query, and the
         probabilities of P c_kv, as bf16 hi/lo pairs instead of rounding them to bf16
         (MLA_FLAG_QC_HILO / MLA_FLAG_P_HILO), closer to the reference's fp32 q_c and P
         (reference_decode.py:250-253) at the cost of more tensor-core issue in K2."""
@@ -101,6 +110,11 @@ class MlaDecodeAttention:
         if (qc_hilo or p_hilo) and self.flags:
             raise ValueError("qc_hilo / p_hilo exist in the default (mma) kernel only")
         self.flags |= (native.FLAG_QC_HILO if qc_hilo else 0) | (native.FLAG_P_HILO if p_hilo else 0)
+        if window < 0 or sinks < 0 or (sinks and not window):
+            raise ValueError("window and sinks must not be negative, and sinks need a window")
+        if window and (check_kernel or kernel == "tcgen05"):
+            raise ValueError("a window exists in the default kernels only")
+        self.window, self.sinks = int(window), int(sinks)
         self.error_word = torch.zeros(1, dtype=torch.int32, device=dev)
         # pinned host copy of the error word: the kernels store a code into it when they
         # record one (MlaDecodeParams.error_host), so the host sees a failed step
@@ -146,6 +160,10 @@ class MlaDecodeAttention:
         p.error_host = _ptr(self.error_host)
         p.num_ctas = self.num_ctas
         p.flags = self.flags | (0 if new_row else native.FLAG_NO_NEW_ROW)
+        if isinstance(cache, PagedLatentCache8):
+            p.flags |= native.FLAG_KV8
+            p.kv_scales = _ptr(cache.scales)
+        p.window, p.sinks = self.window, self.sinks
         p.rope_pos = _ptr(rope_pos)
         p.shard_out = _ptr(shard_out)
         if exchange is not None:
@@ -211,8 +229,8 @@ class MlaDecodeAttention:
         key = (q.data_ptr(), _row_stride(q), kv_a.data_ptr(), _row_stride(kv_a), cache.pages.data_ptr(),
                cache.block_table.data_ptr(), cache.seq_lens.data_ptr(), cache.n_pages, cache.max_blocks,
                q.shape[0], _ptr(out), None if out is None else _row_stride(out), _ptr(rope_pos), _ptr(shard_out),
-               new_row, self.flags, self.num_ctas, self.cos.data_ptr(), self.cos.shape[0], self.kv_b.data_ptr(),
-               None if exchange is None else exchange.key)
+               new_row, self.flags, self.num_ctas, self.window, self.sinks, _scales_ptr(cache), self.cos.data_ptr(),
+               self.cos.shape[0], self.kv_b.data_ptr(), None if exchange is None else exchange.key)
         p = self._step_p
         if key != self._step_key or self._ws is None or p.workspace != self._ws.data_ptr():
             p = self.params(q, kv_a, cache, out, rope_pos=rope_pos, shard_out=shard_out, new_row=new_row,
@@ -237,8 +255,8 @@ class MlaDecodeAttention:
                               device=self.device)
         key = ("x", x_n.data_ptr(), _row_stride(x_n), cache.pages.data_ptr(), cache.block_table.data_ptr(),
                cache.seq_lens.data_ptr(), cache.n_pages, cache.max_blocks, x_n.shape[0], out.data_ptr(),
-               _row_stride(out), self.flags, self.num_ctas, self.cos.data_ptr(), self.cos.shape[0],
-               self.kv_b.data_ptr())
+               _row_stride(out), self.flags, self.num_ctas, self.window, self.sinks, _scales_ptr(cache),
+               self.cos.data_ptr(), self.cos.shape[0], self.kv_b.data_ptr())
         p = self._step_p
         if key != self._step_key or self._ws is None or p.workspace != self._ws.data_ptr():
             p = self.params(None, None, cache, out, x_n=x_n)

@@ -27,12 +27,22 @@ cudaError_t launch_combine_shards(const float* parts, int n_shards, int batch, v
 cudaError_t launch_exchange_combine(const MlaDecodeParams& p, cudaStream_t stream);
 cudaError_t launch_attention_mma(const MlaDecodeParams& p, const CUtensorMap& tmap_kv, float scale_log2,
                                  int sm_count, cudaStream_t stream);
+cudaError_t launch_attention_kv8(const MlaDecodeParams& p, const CUtensorMap& tmap_c, const CUtensorMap& tmap_r,
+                                 float scale_log2, cudaStream_t stream);
+cudaError_t k2_kv8_configure();
 cudaError_t k2_configure();
 cudaError_t k2_mma_configure();
 cudaError_t k3_configure();
 int k3_w_rows(int batch);
 cudaError_t k0_configure();
 cudaError_t launch_rows_to_pages(const MlaRowsToPages& r, int sm_count, cudaStream_t stream);
+uint64_t pool_scratch_bytes(int batch, int n_pages, int max_blocks);
+cudaError_t launch_pool_fork(const MlaPagePool& p, const int32_t* src, const int32_t* dst, int n, cudaStream_t s);
+cudaError_t launch_pool_release(const MlaPagePool& p, const int32_t* requests, int n, cudaStream_t s);
+cudaError_t launch_pool_reserve(const MlaPagePool& p, const int32_t* requests, int n, int tokens, cudaStream_t s);
+cudaError_t launch_pool_compact(const MlaPagePool& p, int sm_count, cudaStream_t s);
+cudaError_t launch_copy_pages(const MlaPagePool& to, const MlaPagePool& from, const int32_t* src, const int32_t* dst,
+                              int n, int sm_count, cudaStream_t s);
 cudaError_t launch_o_proj(const MlaDecodeParams& p, const CUtensorMap& tmap_w, const CUtensorMap& tmap_x,
                           cudaStream_t stream);
 cudaError_t launch_project(const MlaDecodeParams& p, __nv_bfloat16* qkv, const CUtensorMap& tmap_w,
@@ -68,7 +78,8 @@ int device_info(int* sm_count) {
         if (cudaGetDeviceProperties(&prop, dev) != cudaSuccess) { d.status = MLA_E_LAUNCH; return; }
         if (prop.major != 10) { d.status = MLA_E_ARCH; return; }
         if (k0_configure() != cudaSuccess || k0w_configure() != cudaSuccess || k1_configure() != cudaSuccess ||
-            k2_configure() != cudaSuccess || k2_mma_configure() != cudaSuccess || k3_configure() != cudaSuccess) {
+            k2_configure() != cudaSuccess || k2_mma_configure() != cudaSuccess ||
+            k2_kv8_configure() != cudaSuccess || k3_configure() != cudaSuccess) {
             d.status = MLA_E_LAUNCH;
             return;
         }
@@ -110,6 +121,32 @@ int make_tmap_blocks(CUtensorMap* m, const void* base, uint64_t rows_or_pages, b
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? MLA_OK : MLA_E_DRIVER;
+}
+
+// The pages of an 8-bit cache (MLA_PAGE8_BYTES each). Latent part: dims {128 bytes,
+// 8 rows (pitch 512), 4 column blocks (128), 8 groups of 8 rows (4096), pages}, one box
+// per page = 32 KB landing as [8 groups][4 column blocks][8 rows][128 B] with the
+// 128-byte swizzle. Rotary part: dims {64 bytes, 64 rows, pages} behind it, one box
+// per page = 4 KB landing as [64 rows][64 B] with the 64-byte swizzle.
+int make_tmap_kv8(CUtensorMap* c, CUtensorMap* r, void* base, uint64_t n_pages) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn;
+    if (encode_fn(&fn) != MLA_OK) return MLA_E_DRIVER;
+    const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+    const cuuint64_t cdims[5] = {128, 8, kLora / 128, kPage / 8, n_pages};
+    const cuuint64_t cstrides[4] = {kLora, 128, 8 * kLora, MLA_PAGE8_BYTES};
+    const cuuint32_t cbox[5] = {128, 8, kLora / 128, kPage / 8, 1};
+    if (fn(c, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, base, cdims, cstrides, cbox, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return MLA_E_DRIVER;
+    const cuuint64_t rdims[3] = {kRope, kPage, n_pages};
+    const cuuint64_t rstrides[2] = {kRope, MLA_PAGE8_BYTES};
+    const cuuint32_t rbox[3] = {kRope, kPage, 1};
+    return fn(r, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, static_cast<char*>(base) + kPage * kLora, rdims, rstrides, rbox,
+              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+               ? MLA_OK
+               : MLA_E_DRIVER;
 }
 
 // kv_b (16*256 rows x 512 bf16) as row blocks of W_UK / W_UV: dims {64 columns,
@@ -267,14 +304,14 @@ bool aligned(const void* ptr, uintptr_t a) { return (reinterpret_cast<uintptr_t>
 
 // CTAs of the split plan: p->num_ctas, or by default as many as run at once:
 // two per SM for the m16n8k16 kernel (each of its CTAs runs two plan CTAs as
-// independent warp groups) and the checker, one per SM for the tcgen05 kernel.
+// independent warp groups) and the checker, one per SM for the tcgen05 kernels.
 int resolve_ctas(const MlaDecodeParams* p, int* ctas) {
     if (p->num_ctas < 0 || p->num_ctas > kMaxCtas) return MLA_E_LIMIT;
     if (p->num_ctas > 0) { *ctas = p->num_ctas; return MLA_OK; }
     int sms = 0;
     const int st = device_info(&sms);
     if (st != MLA_OK) return st;
-    *ctas = (p->flags & MLA_FLAG_TCGEN05) ? sms : 2 * sms;
+    *ctas = (p->flags & (MLA_FLAG_TCGEN05 | MLA_FLAG_KV8)) ? sms : 2 * sms;
     return MLA_OK;
 }
 
@@ -288,6 +325,57 @@ int check_header(const MlaDecodeParams* p) {
     if (p->batch > MLA_MAX_BATCH) return MLA_E_LIMIT;
     return MLA_OK;
 }
+
+// A caller's error_host, as the device addresses it: pinned host memory that the device can store into.
+int device_error_host(int32_t* host, int32_t** dev) {
+    *dev = nullptr;
+    if (!host) return MLA_OK;
+    if (!aligned(host, 4)) return MLA_E_MISALIGNED;
+    cudaPointerAttributes a;
+    if (cudaPointerGetAttributes(&a, host) != cudaSuccess || a.type != cudaMemoryTypeHost || !a.devicePointer) {
+        cudaGetLastError();
+        return MLA_E_INVALID_ARG;
+    }
+    *dev = static_cast<int32_t*>(a.devicePointer);
+    return MLA_OK;
+}
+
+// The parts of a page pool that copies use.
+int check_pool_pages(const MlaPagePool* p) {
+    if (!p || p->struct_size != sizeof(MlaPagePool) || p->abi_version != MLA_ABI_VERSION) return MLA_E_INVALID_ARG;
+    if (p->n_layers <= 0 || p->n_pages <= 0 || (p->kv8 != 0 && p->kv8 != 1)) return MLA_E_INVALID_ARG;
+    if (p->n_layers > MLA_MAX_LAYERS || (int64_t)p->n_pages * MLA_PAGE_SIZE > INT32_MAX) return MLA_E_LIMIT;
+    for (int l = 0; l < p->n_layers; ++l) {
+        if (!p->pages[l] || (p->kv8 && !p->scales[l])) return MLA_E_INVALID_ARG;
+        if (!aligned(p->pages[l], 16) || !aligned(p->scales[l], 8)) return MLA_E_MISALIGNED;
+    }
+    return MLA_OK;
+}
+
+int check_pool_dims(const MlaPagePool* p) {
+    if (!p || p->struct_size != sizeof(MlaPagePool) || p->abi_version != MLA_ABI_VERSION || p->batch <= 0 ||
+        p->max_blocks <= 0 || p->n_pages <= 0)
+        return MLA_E_INVALID_ARG;
+    if (p->batch > MLA_MAX_BATCH || (int64_t)p->batch * p->max_blocks > INT32_MAX) return MLA_E_LIMIT;
+    return MLA_OK;
+}
+
+// A pool for a call that changes it; fills `out` with the device's view of error_host.
+int prepare_pool(const MlaPagePool* p, MlaPagePool* out) {
+    int st = check_pool_dims(p);
+    if (st != MLA_OK) return st;
+    st = check_pool_pages(p);
+    if (st != MLA_OK) return st;
+    if (!p->block_table || !p->seq_lens || !p->held || !p->refs || !p->scratch) return MLA_E_INVALID_ARG;
+    if (!aligned(p->refs, 16) || !aligned(p->scratch, 256)) return MLA_E_MISALIGNED;
+    if (p->scratch_bytes < pool_scratch_bytes(p->batch, p->n_pages, p->max_blocks)) return MLA_E_WORKSPACE;
+    st = device_info(nullptr);
+    if (st != MLA_OK) return st;
+    *out = *p;
+    return device_error_host(p->error_host, &out->error_host);
+}
+
+int launched(cudaError_t e) { return e == cudaSuccess ? MLA_OK : MLA_E_LAUNCH; }
 
 // Full validation for the launch paths; fills `out` with num_ctas resolved.
 int prepare(const MlaDecodeParams* p, MlaDecodeParams* out) {
@@ -310,10 +398,18 @@ int prepare(const MlaDecodeParams* p, MlaDecodeParams* out) {
         if (!aligned(p->x_n, 16) || (p->x_stride & 7) || !aligned(p->w_qkv, 16)) return MLA_E_MISALIGNED;
     }
     if (p->flags & ~(MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_NO_NEW_ROW | MLA_FLAG_EXCHANGE_SPLIT |
-                     MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO))
+                     MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO | MLA_FLAG_KV8))
         return MLA_E_INVALID_ARG;
     if ((p->flags & (MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO)) && (p->flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05)))
         return MLA_E_INVALID_ARG;  // the hi/lo forms exist in the default kernel only
+    const bool kv8 = (p->flags & MLA_FLAG_KV8) != 0;
+    if (kv8 != (p->kv_scales != nullptr)) return MLA_E_INVALID_ARG;
+    if (kv8 && (p->flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO)))
+        return MLA_E_INVALID_ARG;  // an 8-bit cache has its own split-KV kernel, without these forms
+    if (p->window < 0 || p->sinks < 0 || (p->sinks > 0 && p->window == 0)) return MLA_E_INVALID_ARG;
+    if (p->window > 0 && ((p->flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_NO_NEW_ROW)) ||
+                          p->shard_out || p->world != 0))
+        return MLA_E_INVALID_ARG;  // a window counts from the new row, which a shard need not hold
     if (p->world < 0 || p->world > MLA_MAX_RANKS) return MLA_E_INVALID_ARG;
     if (p->world > 0) {  // peer exchange: K3 writes every rank's buffer, K4 combines into out
         if (p->rank < 0 || p->rank >= p->world || p->shard_out || !p->out || p->exchange_timeout_us < 0)
@@ -334,22 +430,14 @@ int prepare(const MlaDecodeParams* p, MlaDecodeParams* out) {
     if (!aligned(p->kv_cache, 16) || !aligned(p->kv_b, 16) || !aligned(p->workspace, 256) ||
         !aligned(p->q, 4) || (p->q_stride & 1) || (p->out_stride & 1) || !aligned(p->kv_a, 2) || !aligned(p->out, 4) || !aligned(p->kv_a_norm_w, 2) ||
         !aligned(p->rope_cos, 4) || !aligned(p->rope_sin, 4) || !aligned(p->rope_pos, 4) ||
-        !aligned(p->shard_out, 16))
+        !aligned(p->shard_out, 16) || !aligned(p->kv_scales, 8))
         return MLA_E_MISALIGNED;
     int sms = 0;
     st = device_info(&sms);
     if (st != MLA_OK) return st;
     *out = *p;
-    if (p->error_host) {  // must be pinned host memory that the device can store into
-        if (!aligned(p->error_host, 4)) return MLA_E_MISALIGNED;
-        cudaPointerAttributes a;
-        if (cudaPointerGetAttributes(&a, p->error_host) != cudaSuccess || a.type != cudaMemoryTypeHost ||
-            !a.devicePointer) {
-            cudaGetLastError();
-            return MLA_E_INVALID_ARG;
-        }
-        out->error_host = static_cast<int32_t*>(a.devicePointer);
-    }
+    st = device_error_host(p->error_host, &out->error_host);
+    if (st != MLA_OK) return st;
     st = resolve_ctas(p, &out->num_ctas);
     if (st != MLA_OK) return st;
     const WsLayout ws = ws_layout(*out);
@@ -373,6 +461,12 @@ int run_attention(const MlaDecodeParams& q, cudaStream_t s) {
     const float scale_log2 = (float)((double)q.softmax_scale * 1.4426950408889634);
     if (q.flags & MLA_FLAG_CHECK_KERNEL) {
         return launch_attention_check(q, scale_log2, s) == cudaSuccess ? MLA_OK : MLA_E_LAUNCH;
+    }
+    if (q.flags & MLA_FLAG_KV8) {
+        CUtensorMap tc8, tr8;
+        const int st = make_tmap_kv8(&tc8, &tr8, q.kv_cache, (uint64_t)q.n_pages);
+        if (st != MLA_OK) return st;
+        return launch_attention_kv8(q, tc8, tr8, scale_log2, s) == cudaSuccess ? MLA_OK : MLA_E_LAUNCH;
     }
     CUtensorMap tkv, tq;
     const bool tc = (q.flags & MLA_FLAG_TCGEN05) != 0;
@@ -421,6 +515,8 @@ const char* mla_device_error_string(int code) {
         case MLA_DEV_BAD_PAGE: return "block_table entry outside [0, n_pages)";
         case MLA_DEV_BAD_POSITION: return "seq_lens entry outside the rope table or block table";
         case MLA_DEV_TIMEOUT: return "on-chip pipeline wait timed out";
+        case MLA_DEV_NO_PAGE: return "page pool: too few free pages";
+        case MLA_DEV_BAD_REQUEST: return "page pool: request outside the batch, or a destination named twice";
         case MLA_DEV_PEER_TIMEOUT: return "shard exchange: a peer's flag did not arrive in time";
         default: return "unknown device error";
     }
@@ -447,7 +543,7 @@ int mla_workspace_size(const MlaDecodeParams* p, uint64_t* bytes) {
     int ctas = 0;
     st = resolve_ctas(p, &ctas);
     if (st != MLA_OK) return st;
-    *bytes = ws_layout(p->batch, ctas, p->x_n != nullptr, (p->flags & MLA_FLAG_QC_HILO) != 0).total;
+    *bytes = ws_layout(p->batch, ctas, p->x_n != nullptr, stores_q_lo(*p)).total;
     return MLA_OK;
 }
 
@@ -458,7 +554,7 @@ int mla_plan_info(const MlaDecodeParams* p, int32_t* num_ctas, int32_t* num_slot
     st = resolve_ctas(p, &ctas);
     if (st != MLA_OK) return st;
     if (num_ctas) *num_ctas = ctas;
-    if (num_slots) *num_slots = ws_layout(p->batch, ctas, p->x_n != nullptr, (p->flags & MLA_FLAG_QC_HILO) != 0).slots;
+    if (num_slots) *num_slots = ws_layout(p->batch, ctas, p->x_n != nullptr, stores_q_lo(*p)).slots;
     return MLA_OK;
 }
 
@@ -496,12 +592,83 @@ int mla_rows_to_pages(const MlaRowsToPages* r, void* stream) {
                                     !(r->rms_eps >= 0.f)))
         return MLA_E_INVALID_ARG;
     if (!aligned(r->rows, 16) || (r->rows_stride & 7) || !aligned(r->kv_cache, 16) || !aligned(r->row_start, 8) ||
-        !aligned(r->kv_a_norm_w, 2) || !aligned(r->rope_cos, 4) || !aligned(r->rope_sin, 4))
+        !aligned(r->kv_a_norm_w, 2) || !aligned(r->rope_cos, 4) || !aligned(r->rope_sin, 4) ||
+        !aligned(r->kv_scales, 8))
         return MLA_E_MISALIGNED;
     int sms = 0;
     const int st = device_info(&sms);
     if (st != MLA_OK) return st;
     return launch_rows_to_pages(*r, sms, (cudaStream_t)stream) == cudaSuccess ? MLA_OK : MLA_E_LAUNCH;
+}
+
+void mla_pool_init(MlaPagePool* p) {
+    if (!p) return;
+    *p = MlaPagePool{};
+    p->struct_size = sizeof(MlaPagePool);
+    p->abi_version = MLA_ABI_VERSION;
+}
+
+int mla_pool_scratch_size(const MlaPagePool* p, uint64_t* bytes) {
+    if (!bytes) return MLA_E_INVALID_ARG;
+    const int st = check_pool_dims(p);
+    if (st != MLA_OK) return st;
+    *bytes = pool_scratch_bytes(p->batch, p->n_pages, p->max_blocks);
+    return MLA_OK;
+}
+
+int mla_pool_fork(const MlaPagePool* p, const int32_t* src, const int32_t* dst, int32_t n, void* stream) {
+    MlaPagePool q;
+    const int st = prepare_pool(p, &q);
+    if (st != MLA_OK) return st;
+    if (n < 0 || (n > 0 && (!src || !dst))) return MLA_E_INVALID_ARG;
+    if (n > q.batch) return MLA_E_LIMIT;  // more pairs than destinations
+    return n == 0 ? MLA_OK : launched(launch_pool_fork(q, src, dst, n, (cudaStream_t)stream));
+}
+
+int mla_pool_release(const MlaPagePool* p, const int32_t* requests, int32_t n, void* stream) {
+    MlaPagePool q;
+    const int st = prepare_pool(p, &q);
+    if (st != MLA_OK) return st;
+    if (n < 0 || (n > 0 && !requests)) return MLA_E_INVALID_ARG;
+    if (n > q.batch) return MLA_E_LIMIT;
+    return n == 0 ? MLA_OK : launched(launch_pool_release(q, requests, n, (cudaStream_t)stream));
+}
+
+int mla_pool_reserve(const MlaPagePool* p, const int32_t* requests, int32_t n, int32_t tokens, void* stream) {
+    MlaPagePool q;
+    const int st = prepare_pool(p, &q);
+    if (st != MLA_OK) return st;
+    if (!requests) n = q.batch;
+    if (n < 0 || tokens < 0) return MLA_E_INVALID_ARG;
+    if (n > q.batch) return MLA_E_LIMIT;
+    return n == 0 ? MLA_OK : launched(launch_pool_reserve(q, requests, n, tokens, (cudaStream_t)stream));
+}
+
+int mla_pool_compact(const MlaPagePool* p, void* stream) {
+    MlaPagePool q;
+    int st = prepare_pool(p, &q);
+    if (st != MLA_OK) return st;
+    int sms = 0;
+    st = device_info(&sms);
+    if (st != MLA_OK) return st;
+    return launched(launch_pool_compact(q, sms, (cudaStream_t)stream));
+}
+
+int mla_copy_pages(const MlaPagePool* to, const MlaPagePool* from, const int32_t* src, const int32_t* dst, int32_t n,
+                   void* stream) {
+    int st = check_pool_pages(to);
+    if (st != MLA_OK) return st;
+    st = check_pool_pages(from);
+    if (st != MLA_OK) return st;
+    if (n < 0 || (n > 0 && (!src || !dst)) || to->n_layers != from->n_layers || to->kv8 != from->kv8)
+        return MLA_E_INVALID_ARG;
+    int sms = 0;
+    st = device_info(&sms);
+    if (st != MLA_OK) return st;
+    MlaPagePool q = *to;
+    st = device_error_host(to->error_host, &q.error_host);
+    if (st != MLA_OK) return st;
+    return n == 0 ? MLA_OK : launched(launch_copy_pages(q, *from, src, dst, n, sms, (cudaStream_t)stream));
 }
 
 int mla_project(const MlaDecodeParams* p, void* stream) {

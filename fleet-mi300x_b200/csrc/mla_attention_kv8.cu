@@ -1,0 +1,730 @@
+// K2 over an 8-bit latent cache — split-KV absorbed-MLA attention on tcgen05.mma
+// kind::f8f6f4, with the scores and the output in tensor memory.
+//
+// Per request, with e4m3 rows C_t (latent c_t, rotary k_t) under the block scales
+// 2^ec_t, 2^er_t:
+//   s_t[h] = softmax_scale (2^ec_t q_c[h] . c_t + 2^er_t q_pe[h] . k_t)
+//   o[h]   = sum_t softmax(s)_t 2^ec_t c_t
+//
+// Why tensor memory here and m16n8k16 on the bf16 cache: with half the bytes per row
+// the SM has half the time per row (25 clocks at the copy peak), and m16n8k16 would
+// spend 70 % of its issue on it before a single conversion. An f8f6f4 MMA takes a
+// tile of 128 tokens x 32 bytes whatever its N (measured: 60 clocks per issued MMA at
+// N = 16 and N = 32, M = 64 and 128, one issuing thread), so 128 tokens x 16 heads
+// cost 18 + 16 MMAs, which two issuing threads keep under a third of the tile's HBM
+// time (about 3,300 clocks). N is nearly free, so it carries precision: an operand
+// that is not 8 bits already enters as a pair of e4m3 values side by side on N,
+// x = hi + lo / 16, about as precise as bf16 (8 significant bits):
+//   scores  S^T[t][hi 16 | lo 16]  = C[t][:] . Q[hi | lo]   (latent and rotary apart: their scales differ)
+//   output  O^T[l][hi 16 | lo 16] += C^T[l][t] P^T[t][hi | lo]
+// The same tile bytes are the K-major A operand of the scores and the MN-major A
+// operand of the output.
+//
+// The scale of a row enters its probability: P'_t = 2^(s_t + ec_t - m) with m a
+// running reference for the largest s_t + ec_t, and the row sum takes
+// P'_t 2^-ec_t. P' lies in [0, 256]; a typical largest one is 16, so that a
+// later score may exceed the reference 16-fold before the output is rescaled (the
+// rescale reads and writes O in tensor memory, which happens in the first few tiles
+// of a segment only). Sums, scores and the output are fp32.
+//
+// Tiles of up to two 64-row pages of a request (the plan's units are pages), TMA'd
+// into a ring of two; rows that the query does not see have P' = 0 and, if they share
+// a 32-row step with visible ones, are zeroed in the tile (0 times stale NaN bytes
+// would be NaN).
+//
+// Warps (512 threads):
+//   0      TMA producer: lanes 0 and 1 each load one page of the tile and its exponents
+//   1      score MMAs, owns the tensor memory
+//   2      output MMAs
+//   4-11   softmax: one token and eight heads per thread; partials of a finished segment
+//   12-15  the query of the next segment: e4m3 pairs under one scale per part
+// The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
+// descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
+// clocks of moving them there, elected it takes the 40 that its operands' shared-memory
+// reads need (5 KB at 128 B per clock).
+// Every wait is bounded: a stall records MLA_DEV_TIMEOUT, the roles fall through
+// their remaining waits, copies and MMAs drain and the tensor memory is freed.
+#include <cuda.h>
+
+#include "mla_kv8.cuh"
+#include "mla_tiles.cuh"
+
+namespace mla {
+
+namespace kv8 {
+
+constexpr int kThreads = 512;
+constexpr int kSmWarps = 8;                     // softmax warps: 4 token quarters x 2 halves of the heads
+constexpr int kSmThreads = kSmWarps * 32;
+constexpr int kHh = kHeads / 2;                 // heads of a softmax thread
+constexpr int kStages = 2;
+constexpr int kTok = 2 * kPage;                 // tokens per tile
+constexpr int kGroup = 8 * kLora;               // 4096: 8 rows of the latent part, [4 column blocks][8][128 B]
+constexpr int kHalfC = kPage * kLora;           // one page's latent bytes in a stage
+constexpr int kHalfR = kPage * kRope;
+constexpr int kStageC = 2 * kHalfC;             // 65,536
+constexpr int kStageR = 2 * kHalfR;             // 8,192
+constexpr int kN = 2 * kHeads;                  // hi | lo
+constexpr int kQC = kN * kLora;                 // [4 column blocks][32][128 B]
+constexpr int kQR = kN * kRope;                 // [32][64 B]
+constexpr int kP = kTok * kN;                   // [128 tokens][32 B]
+
+constexpr int kOffC = 0;
+constexpr int kOffR = kOffC + kStages * kStageC;
+constexpr int kOffQC = kOffR + kStages * kStageR;
+constexpr int kOffQR = kOffQC + 2 * kQC;
+constexpr int kOffP = kOffQR + 2 * kQR;
+constexpr int kOffMisc = kOffP + 2 * kP;
+
+struct Smem {
+    uint64_t full[kStages], empty[kStages][2];
+    uint64_t q_full[2], q_empty[2];
+    uint64_t s_full[2], p_full[2], pv_done[2];
+    uint64_t o_empty, teardown[2];
+    uint64_t exps[kStages][2];  // a page's 4 x 2 exponents
+    float q_scale[2][2];        // [buffer][part]: what the pair was divided by
+    float q_red[4][2];
+    float red[2][4][16];
+    float lred[4][16];
+    uint32_t tmem_base;
+    int abort;
+};
+constexpr int kSmemBytes = kOffMisc + (int)sizeof(Smem) + 1024;  // + alignment slack
+static_assert(kSmemBytes <= 232448, "K2 (8-bit) shared memory exceeds 227 KB");
+static_assert(kOffP % 1024 == 0 && kOffQR % 1024 == 0, "operands must stay 1024-byte aligned");
+
+// Tensor memory columns: two score buffers (latent 32 | rotary 32), four output blocks.
+constexpr int kTmemS = 0, kTmemO = 128, kTmemCols = 256;
+
+// Instruction descriptor of kind::f8f6f4 with e4m3 A/B and fp32 D (the fields of
+// idesc_bf16_f32; format 0 = e4m3).
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, int a_mn_major, int b_mn_major) {
+    return (1u << 4) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) |
+           (uint32_t(M >> 4) << 24);
+}
+constexpr uint32_t kIdescQK = idesc_e4m3(128, kN, 0, 0);
+constexpr uint32_t kIdescPV = idesc_e4m3(128, kN, 1, 1);
+
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Shared-memory descriptor as smem_desc_sw128, with the layout (swizzle) given: 2 =
+// 128-byte, 4 = 64-byte, 6 = 32-byte; sbo: bytes between groups of 8 rows (K-major)
+// or of 8 k (MN-major).
+constexpr int kSw128 = 2, kSw64 = 4, kSw32 = 6;
+__device__ __forceinline__ uint64_t desc_of(uint32_t saddr, uint32_t sbo_bytes, int layout) {
+    return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3FFF) << 32) |
+           (uint64_t(1) << 46) | (uint64_t(layout) << 61);
+}
+
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const void* tmap, uint64_t* bar, int x, int y, int z,
+                                            int w, int v, uint64_t cache_hint) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v),
+        "l"(cache_hint)
+        : "memory");
+}
+
+// A CTA's tiles: one or two plan units (pages) of one request.
+struct Walk : TileCursor {
+    __device__ int pages() const { return u + 1 < u_end && u + 1 < cb1 ? 2 : 1; }
+    __device__ bool last() const { return u + pages() == u_end || u + pages() == cb1; }
+    __device__ void next() {
+        u += pages() - 1;
+        TileCursor::next();
+    }
+    __device__ void next_request() {
+        u = min(cb1, u_end) - 1;
+        TileCursor::next();
+    }
+};
+
+// Whether any row of the tile's 32-row step ks is visible.
+__device__ __forceinline__ bool step_on(const Visible& v, int index, int pages, int ks) {
+    if ((ks >> 1) >= pages) return false;
+    const int r0 = kPage * v.tile(index + (ks >> 1)) + 32 * (ks & 1);
+    return r0 < v.rows && (r0 < v.head || r0 + 32 > v.lo);
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(r));
+    return r != 0;
+}
+
+// 32 lanes x 8 consecutive tensor-memory columns (tmem_ld16, half as wide), and back.
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[kHh]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr));
+}
+// The loaded values, not to be used before the tmem_wait_ld that precedes this call.
+__device__ __forceinline__ void loaded(float (&v)[kHh]) {
+    asm volatile("" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[kHh]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+                 "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+                 : "memory");
+}
+
+// Reduction of 8 values over the 32 lanes of a warp by halving exchanges: lanes 4 h ..
+// 4 h + 3 end with value h.
+template <bool kMax>
+__device__ __forceinline__ float reduce8(const float (&v)[kHh], int lane) {
+    auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
+    float r4[4], r2[2];
+    const bool b4 = lane & 16, b3 = lane & 8, b2 = lane & 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float send = b4 ? v[j] : v[j + 4], keep = b4 ? v[j + 4] : v[j];
+        r4[j] = op(keep, __shfl_xor_sync(0xffffffffu, send, 16));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const float send = b3 ? r4[j] : r4[j + 2], keep = b3 ? r4[j + 2] : r4[j];
+        r2[j] = op(keep, __shfl_xor_sync(0xffffffffu, send, 8));
+    }
+    const float send = b2 ? r2[0] : r2[1], keep = b2 ? r2[1] : r2[0];
+    float r = op(keep, __shfl_xor_sync(0xffffffffu, send, 4));
+    r = op(r, __shfl_xor_sync(0xffffffffu, r, 2));
+    return op(r, __shfl_xor_sync(0xffffffffu, r, 1));
+}
+
+}  // namespace kv8
+
+__global__ void __launch_bounds__(kv8::kThreads, 1)
+    k2_attention_kv8(const MlaDecodeParams p, const __grid_constant__ CUtensorMap tmap_c,
+                     const __grid_constant__ CUtensorMap tmap_r, float scale_log2) {
+    using namespace kv8;
+    MLA_TL_SCOPE(1);
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    Smem& S = *reinterpret_cast<Smem*>(smem + kOffMisc);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+    const WsLayout ws = ws_layout(p);
+    char* wsb = reinterpret_cast<char*>(p.workspace);
+    const ErrSink err = err_sink(p);
+    const int fresh = new_row_count(p);
+
+    pdl_trigger();
+    const int vc = blockIdx.x;
+
+    // The split plan: for up to 64 requests from the step's inputs, before the wait on K1
+    // (the rule K1's planner uses); beyond, K1's plan entry after it.
+    constexpr int kPrePlan = 64;
+    __shared__ int32_t pre_cum[kPrePlan + 1];
+    __shared__ int32_t pre_tot[2];
+    const bool pre = p.batch <= kPrePlan;
+    const int32_t* cum = reinterpret_cast<const int32_t*>(wsb + ws.tiles_cum);
+    PlanEntry pe{};
+    int G = 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&S.full[i], 2);
+            mbar_init(&S.empty[i][0], 1);
+            mbar_init(&S.empty[i][1], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&S.q_full[i], 128);
+            mbar_init(&S.q_empty[i], 1 + kSmWarps);
+            mbar_init(&S.s_full[i], 1);
+            mbar_init(&S.p_full[i], kSmThreads);
+            mbar_init(&S.pv_done[i], 1);
+            mbar_init(&S.teardown[i], 1);
+        }
+        mbar_init(&S.o_empty, kSmThreads);
+        S.abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmap_c);
+        prefetch_tmap(&tmap_r);
+    }
+    if (pre) {
+        int n = 0, incl = 0;
+        if (threadIdx.x < kPrePlan) {
+            n = (int)threadIdx.x < p.batch ? plan_tiles(p, threadIdx.x) : 0;
+            incl = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            if (lane == 31) pre_tot[warp] = incl;
+        }
+        __syncthreads();
+        if (threadIdx.x < kPrePlan) {
+            const int before = warp ? pre_tot[0] : 0;
+            pre_cum[threadIdx.x] = before + incl - n;  // beyond the batch: the total
+            if (threadIdx.x == kPrePlan - 1) pre_cum[kPrePlan] = before + incl;
+        }
+        __syncthreads();
+        cum = pre_cum;
+        const int64_t U = pre_cum[p.batch];
+        G = (int)(U < (int64_t)p.num_ctas ? U : (int64_t)p.num_ctas);
+        if (vc < G) {
+            pe.u_begin = plan_begin(vc, U, G);
+            pe.u_end = plan_begin(vc + 1, U, G);
+            int lo = 0, hi = p.batch;  // largest b with cum[b] <= u_begin (skips empty requests)
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (pre_cum[mid] <= pe.u_begin) lo = mid; else hi = mid;
+            }
+            pe.b = lo;
+            pe.cb0 = pre_cum[lo];
+            pe.cb1 = pre_cum[lo + 1];
+        }
+    } else {
+        __syncthreads();  // barriers initialised
+        pdl_wait();
+        MLA_TL_WAITED(1);
+        G = reinterpret_cast<const PlanHeader*>(wsb + ws.plan)->G;
+        pe = reinterpret_cast<const PlanEntry*>(wsb + ws.plan + sizeof(PlanHeader))[vc < G ? vc : 0];
+    }
+    if (vc >= G) {  // uniform per CTA: no work, nothing allocated
+        if (pre) pdl_wait();
+        return;
+    }
+
+    if (warp == 1) { tmem_alloc(&S.tmem_base, kTmemCols); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem_base, 0);
+    volatile int* abort = &S.abort;
+    // A bounded wait; once a role gave up, every other wait falls through at once.
+    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+        return mbar_wait(bar, parity, abort, err);
+    };
+
+    Walk cur;
+    cur.init_at(cum, p.seq_lens, p.batch, pe, fresh);
+    auto visible = [&](int b) { return Visible(p, p.seq_lens[b] + fresh, kPage); };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ producer
+        // Lane l (0, 1) loads page l of each tile. The page id is loaded two tiles ahead
+        // and the exponents one tile ahead, so that neither latency is on the path.
+        if (lane < 2) {
+            Visible vis;
+            auto page_of = [&](const Walk& w) -> int {
+                if (w.first()) vis = visible(w.b);
+                if (!w.valid() || lane >= w.pages()) return -1;  // no page for this lane
+                int pg = p.block_table[(int64_t)w.b * p.max_blocks + vis.tile(w.index() + lane)];
+                if (pg < 0 || pg >= p.n_pages) { record_error(err, MLA_DEV_BAD_PAGE); pg = 0; }
+                return pg;
+            };
+            auto exps_of = [&](int pg) -> uint64_t {
+                return pg < 0 ? 0ull : reinterpret_cast<const uint64_t*>(p.kv_scales)[pg];
+            };
+            uint32_t issued = 0;
+            auto issue = [&](uint32_t j, int pg, uint64_t ex) {
+                const uint32_t st = j % kStages;
+                S.exps[st][lane] = ex;
+                if (pg < 0) {
+                    mbar_arrive(&S.full[st]);
+                } else {
+                    mbar_arrive_expect_tx(&S.full[st], kHalfC + kHalfR);
+                    tma_load_5d(smem + kOffC + st * kStageC + lane * kHalfC, &tmap_c, &S.full[st], 0, 0, 0, 0, pg,
+                                kCacheEvictFirst);
+                    tma_load_3d(smem + kOffR + st * kStageR + lane * kHalfR, &tmap_r, &S.full[st], 0, 0, pg,
+                                kCacheEvictFirst);
+                }
+                ++issued;
+            };
+            int pg0 = page_of(cur);
+            bool early = false;
+            if (pre) {  // the first page before the wait, unless it is the one K1 appends to
+                const bool holds_new = fresh && pg0 >= 0 && vis.tile(cur.index() + lane) == (vis.rows - 1) / kPage;
+                if (!holds_new) {
+                    issue(0, pg0, exps_of(pg0));
+                    early = true;
+                }
+            }
+            Walk la = cur;  // two tiles ahead of the one being loaded
+            la.next();
+            int pg1 = la.valid() ? page_of(la) : -1;
+            if (pre) { pdl_wait(); MLA_TL_WAITED(1); }
+            uint64_t ex0 = exps_of(pg0);
+            uint32_t j = 0;
+            for (; cur.valid(); cur.next(), ++j) {
+                la.next();
+                const int pg2 = la.valid() ? page_of(la) : -1;
+                const uint64_t ex1 = exps_of(pg1);
+                if (!(j == 0 && early)) {
+                    if (j >= kStages && !wait(&S.empty[j % kStages][lane], (j / kStages - 1) & 1)) break;
+                    issue(j, pg0, ex0);
+                }
+                pg0 = pg1; pg1 = pg2; ex0 = ex1;
+            }
+            // Drain: every issued copy must land before the CTA's shared memory is released.
+            for (uint32_t st = 0; st < kStages; ++st) {
+                const uint32_t fills = issued / kStages + (st < issued % kStages ? 1u : 0u);
+                if (fills) mbar_drain(&S.full[st], (fills - 1) & 1, err);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ score MMAs
+        const uint64_t dc = desc_of(smem_u32(smem + kOffC), kGroup, kSw128);
+        const uint64_t dr = desc_of(smem_u32(smem + kOffR), 8 * kRope, kSw64);
+        const uint64_t dqc = desc_of(smem_u32(smem + kOffQC), 1024, kSw128);
+        const uint64_t dqr = desc_of(smem_u32(smem + kOffQR), 8 * kRope, kSw64);
+        uint32_t j = 0;
+        for (; cur.valid(); cur.next(), ++j) {
+            const uint32_t st = j % kStages, qb = cur.seg & 1, sb = j & 1;
+            if (cur.first() && !wait(&S.q_full[qb], (cur.seg >> 1) & 1)) break;
+            if (!wait(&S.full[st], (j / kStages) & 1)) break;
+            if (j >= 2 && !wait(&S.p_full[sb], ((j - 2) >> 1) & 1)) break;  // the buffer's scores were read
+            tc_fence_after();
+            __syncwarp();
+            const uint64_t a = dc + ((st * kStageC) >> 4), b = dqc + ((qb * kQC) >> 4);
+            const uint64_t ar = dr + ((st * kStageR) >> 4), br = dqr + ((qb * kQR) >> 4);
+            const uint32_t d = tmem + kTmemS + 64 * sb;
+            const bool last = cur.last();
+            if (elect_one()) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    mma_f8(d, a + (((i >> 2) * 1024 + (i & 3) * 32) >> 4),
+                           b + (((i >> 2) * (kN * 128) + (i & 3) * 32) >> 4), kIdescQK, i > 0);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    mma_f8(d + kN, ar + ((i * 32) >> 4), br + ((i * 32) >> 4), kIdescQK, i > 0);
+                tc_commit(&S.s_full[sb]);
+                if (last) tc_commit(&S.q_empty[qb]);
+            }
+            __syncwarp();
+        }
+        __syncwarp();
+        if (elect_one()) {  // all issued MMAs complete before the tensor memory is freed
+            tc_commit(&S.teardown[0]);
+            mbar_drain(&S.teardown[0], 0, err);
+        }
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ output MMAs
+        const uint64_t dc = desc_of(smem_u32(smem + kOffC), kGroup, kSw128);
+        const uint64_t dp = desc_of(smem_u32(smem + kOffP), 8 * kN, kSw32);
+        Visible vis;
+        uint32_t j = 0;
+        for (; cur.valid(); cur.next(), ++j) {
+            const uint32_t st = j % kStages, sb = j & 1;
+            const bool first = cur.first();
+            if (first) vis = visible(cur.b);
+            uint32_t on = 0;  // bit ks: the 32-row step ks holds a visible row
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), cur.pages(), ks) << ks;
+            if (!wait(&S.p_full[sb], (j >> 1) & 1)) break;
+            if (first && cur.seg > 0 && !wait(&S.o_empty, (cur.seg - 1) & 1)) break;
+            if (!wait(&S.full[st], (j / kStages) & 1)) break;
+            tc_fence_after();
+            __syncwarp();
+            const uint64_t a = dc + ((st * kStageC) >> 4), b = dp + ((sb * kP) >> 4);
+            if (elect_one()) {
+                uint32_t acc = first ? 0u : 1u;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    if ((on >> ks) & 1) {
+#pragma unroll
+                        for (int cb = 0; cb < 4; ++cb)
+                            mma_f8(tmem + kTmemO + kN * cb, a + ((ks * 4 * kGroup + cb * 1024) >> 4),
+                                   b + ((ks * 32 * kN) >> 4), kIdescPV, acc);
+                        acc = 1u;
+                    }
+                    if (ks & 1) tc_commit(&S.empty[st][ks >> 1]);
+                }
+                tc_commit(&S.pv_done[sb]);
+            }
+            __syncwarp();
+        }
+        __syncwarp();
+        if (elect_one()) {
+            tc_commit(&S.teardown[1]);
+            mbar_drain(&S.teardown[1], 0, err);
+        }
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------ queries
+        // Warp a converts heads 4a .. 4a + 3: lane holds 2 units of 8 latent values per
+        // head and one rotary unit (head 4a + lane / 8, unit lane % 8).
+        if (pre) pdl_wait();
+        const int a = warp - 12;
+        const __nv_bfloat16* qa = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa);
+        const __nv_bfloat16* qa_lo = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa_lo);
+        // 8 values of a bf16 unit, plus its remainders
+        auto unit = [](const uint4& v, float (&x)[8]) {
+            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { x[2 * i] = __low2float(h[i]); x[2 * i + 1] = __high2float(h[i]); }
+        };
+        auto sum = [&](const uint4& v, const uint4& r, float (&x)[8]) {
+            float y[8];
+            unit(v, x);
+            unit(r, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] += y[i];
+        };
+        auto amax8 = [](const float (&x)[8], float m) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[i]));
+            return m;
+        };
+        auto put8 = [](const float (&x)[8], float f, uint8_t* hi, uint8_t* lo) {
+            uint32_t wh[2], wl[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t a2[2], b2[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float u = nan_if_inf(x[4 * i + 2 * k]) * f, w = nan_if_inf(x[4 * i + 2 * k + 1]) * f;
+                    a2[k] = e4m3x2(u, w);
+                    const float2 r = from_e4m3x2(a2[k]);
+                    b2[k] = e4m3x2((u - r.x) * 16.f, (w - r.y) * 16.f);
+                }
+                wh[i] = a2[0] | (a2[1] << 16);
+                wl[i] = b2[0] | (b2[1] << 16);
+            }
+            *reinterpret_cast<uint2*>(hi) = make_uint2(wh[0], wh[1]);
+            *reinterpret_cast<uint2*>(lo) = make_uint2(wl[0], wl[1]);
+        };
+        for (; cur.valid(); cur.next_request()) {
+            const int qb = cur.seg & 1;
+            const __nv_bfloat16* q = qa + (int64_t)cur.b * kQRows * kRow;
+            const __nv_bfloat16* ql = qa_lo + (int64_t)cur.b * kQRows * kLora;
+            uint4 vc4[8], vl4[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                vc4[i] = reinterpret_cast<const uint4*>(q + (4 * a + (i >> 1)) * kRow)[32 * (i & 1) + lane];
+                vl4[i] = reinterpret_cast<const uint4*>(ql + (4 * a + (i >> 1)) * kLora)[32 * (i & 1) + lane];
+            }
+            float xr[8], x[8];
+            unit(reinterpret_cast<const uint4*>(q + (4 * a + (lane >> 3)) * kRow + kLora)[lane & 7], xr);
+            float mc = 0.f, mr = amax8(xr, 0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                sum(vc4[i], vl4[i], x);
+                mc = amax8(x, mc);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1) {
+                mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, o));
+                mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
+            }
+            if (lane == 0) { S.q_red[a][0] = mc; S.q_red[a][1] = mr; }
+            named_bar_sync(2, 128);
+            mc = fmaxf(fmaxf(S.q_red[0][0], S.q_red[1][0]), fmaxf(S.q_red[2][0], S.q_red[3][0]));
+            mr = fmaxf(fmaxf(S.q_red[0][1], S.q_red[1][1]), fmaxf(S.q_red[2][1], S.q_red[3][1]));
+            named_bar_sync(2, 128);  // read before the next segment's values
+            const int ec = scale_exponent(mc), er = scale_exponent(mr);
+            if (cur.seg >= 2) wait(&S.q_empty[qb], ((cur.seg >> 1) - 1) & 1);
+            if (a == 0 && lane == 0) { S.q_scale[qb][0] = pow2i(ec); S.q_scale[qb][1] = pow2i(er); }
+            const float fc = pow2i(-ec), fr = pow2i(-er);
+            uint8_t* qc = smem + kOffQC + qb * kQC;
+            uint8_t* qr = smem + kOffQR + qb * kQR;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int n = 4 * a + (i >> 1), col = 8 * (32 * (i & 1) + lane);  // latent column
+                uint8_t* at = qc + (col >> 7) * (kN * 128) + n * 128 + (((((col & 127) >> 4)) ^ (n & 7)) << 4) + (col & 15);
+                sum(vc4[i], vl4[i], x);
+                put8(x, fc, at, at + kHeads * 128);  // row n + 16 has the same swizzle
+            }
+            {
+                const int n = 4 * a + (lane >> 3), col = 8 * (lane & 7);
+                uint8_t* at = qr + n * kRope + (((col >> 4) ^ ((n >> 1) & 3)) << 4) + (col & 15);
+                put8(xr, fr, at, at + kHeads * kRope);
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(&S.q_full[qb]);
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ softmax, partials
+        const int sp = warp & 3, tok = 32 * sp + lane, half = tok >> 6, slot = tok & (kPage - 1);
+        const int h0 = warp < 8 ? 0 : kHh;  // this thread's heads: h0 .. h0 + 7
+        float* part_ml = reinterpret_cast<float*>(wsb + ws.part_ml);
+        float* part_acc = reinterpret_cast<float*>(wsb + ws.part_acc);
+        if (pre) pdl_wait();   // the previous step's merge has read the partials
+        float m[kHh], l[kHh];  // reference (log2 domain), this thread's part of the row sum
+        float qsc = 0.f, qsr = 0.f;
+        Visible vis;
+        uint32_t j = 0;
+        for (; cur.valid(); cur.next(), ++j) {
+            const uint32_t st = j % kStages, sb = j & 1;
+            const bool first = cur.first(), last = cur.last();
+            if (first) vis = visible(cur.b);
+            const int index = cur.index(), pages = cur.pages();
+            const bool sees = half < pages && vis.row(kPage * vis.tile(index + half) + slot);
+            wait(&S.full[st], (j / kStages) & 1);  // the exponents, and the tile itself where rows are zeroed
+            const char2 ex = sees ? reinterpret_cast<const char2*>(&S.exps[st][half])[slot / kBlock8] : make_char2(0, 0);
+            if (first) {
+                const int qb = cur.seg & 1;
+                wait(&S.q_full[qb], (cur.seg >> 1) & 1);
+                qsc = S.q_scale[qb][0] * scale_log2;
+                qsr = S.q_scale[qb][1] * scale_log2;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S.q_empty[qb]);
+#pragma unroll
+                for (int h = 0; h < kHh; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
+            }
+            const float fc = pow2i(ex.x) * qsc, fr = pow2i(ex.y) * qsr, e = (float)ex.x;
+            wait(&S.s_full[sb], (j >> 1) & 1);
+            tc_fence_after();
+            __syncwarp();
+            float s[kHh];
+            {
+                float a[kHh], b[kHh], c[kHh];
+                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemS + 64 * sb + h0);
+                tmem_ld8(ta, s);
+                tmem_ld8(ta + 16, a);
+                tmem_ld8(ta + 32, b);
+                tmem_ld8(ta + 48, c);
+                tmem_wait_ld();
+                loaded(s); loaded(a); loaded(b); loaded(c);
+#pragma unroll
+                for (int h = 0; h < kHh; ++h)
+                    s[h] = sees ? fmaf(fmaf(a[h], 0.0625f, s[h]), fc, fmaf(fmaf(c[h], 0.0625f, b[h]), fr, e)) : -INFINITY;
+            }
+            // ---- the reference per head: kept unless a score exceeds it 256-fold (16-fold the
+            // largest so far); the first tile of a segment sets it ----
+            bool exchange = first;
+            if (!first) {
+                bool over = false;
+#pragma unroll
+                for (int h = 0; h < kHh; ++h) over |= s[h] > m[h] + 8.f;
+                exchange = bar_red_or(1, kSmThreads, over);
+            }
+            if (exchange) {
+                const float wmax = reduce8<true>(s, lane);
+                if ((lane & 3) == 0) S.red[sb][sp][h0 + (lane >> 2)] = wmax;
+                named_bar_sync(1, kSmThreads);
+                float f[kHh];
+#pragma unroll
+                for (int h = 0; h < kHh; ++h) {
+                    const float t = fmaxf(fmaxf(S.red[sb][0][h0 + h], S.red[sb][1][h0 + h]),
+                                          fmaxf(S.red[sb][2][h0 + h], S.red[sb][3][h0 + h]));
+                    const float n = fmaxf(m[h], t - 4.f);
+                    f[h] = first ? 1.f : fast_exp2(m[h] - n);
+                    m[h] = n;
+                    l[h] *= f[h];
+                }
+                if (!first) {
+                    wait(&S.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
+                    tc_fence_after();
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {  // four blocks, hi and lo
+                        float o[kHh];
+                        const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + 16 * k + h0);
+                        tmem_ld8(ta, o);
+                        tmem_wait_ld();
+                        loaded(o);
+#pragma unroll
+                        for (int h = 0; h < kHh; ++h) o[h] *= f[h];
+                        tmem_st8(ta, o);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            // ---- P' as e4m3 pairs, the row sums over the unrounded values ----
+            const float back = pow2i(-(int)ex.x);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint32_t x[2], y[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int h = 4 * k + 2 * i;
+                    const float u = sees ? fast_exp2(s[h] - m[h]) : 0.f, w = sees ? fast_exp2(s[h + 1] - m[h + 1]) : 0.f;
+                    l[h] = fmaf(u, back, l[h]);
+                    l[h + 1] = fmaf(w, back, l[h + 1]);
+                    x[i] = e4m3x2(u, w);
+                    const float2 r = from_e4m3x2(x[i]);
+                    y[i] = e4m3x2((u - r.x) * 16.f, (w - r.y) * 16.f);
+                }
+                hi[k] = x[0] | (x[1] << 16);
+                lo[k] = y[0] | (y[1] << 16);
+            }
+            if (j >= 2) wait(&S.pv_done[sb], ((j - 2) >> 1) & 1);  // the P buffer is free
+            {
+                uint8_t* pt = smem + kOffP + sb * kP + tok * kN + h0;
+                const int sw = (tok >> 2) & 1;
+                *reinterpret_cast<uint2*>(pt + (sw << 4)) = make_uint2(hi[0], hi[1]);
+                *reinterpret_cast<uint2*>(pt + ((sw ^ 1) << 4)) = make_uint2(lo[0], lo[1]);
+            }
+            if (!sees && step_on(vis, index, pages, sp)) {  // 0 * stale bytes must be 0
+                uint8_t* row = smem + kOffC + st * kStageC + (tok >> 3) * kGroup + (tok & 7) * 128 + (h0 >> 3) * 2048;
+#pragma unroll 4
+                for (int i = 0; i < kLora / 32; ++i)  // this half's two column blocks
+                    *reinterpret_cast<uint4*>(row + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            tc_fence_before();
+            mbar_arrive(&S.p_full[sb]);
+
+            if (last) {
+                const float ls = reduce8<false>(l, lane);
+                if ((lane & 3) == 0) S.lred[sp][h0 + (lane >> 2)] = ls;
+                named_bar_sync(1, kSmThreads);
+                const int64_t part = (int64_t)vc + cur.b;
+                if (sp == 0 && lane < kHh) {
+                    float mh = 0.f;
+#pragma unroll
+                    for (int h = 0; h < kHh; ++h) if (h == lane) mh = m[h];
+                    const int h = h0 + lane;
+                    const float lh = (S.lred[0][h] + S.lred[1][h]) + (S.lred[2][h] + S.lred[3][h]);
+                    *reinterpret_cast<float2*>(part_ml + (part * kHeads + h) * 2) = make_float2(mh, lh);
+                }
+                __syncwarp();
+                wait(&S.pv_done[sb], (j >> 1) & 1);
+                tc_fence_after();
+                __syncwarp();
+                float* acc = part_acc + (part * kHeads + h0) * kLora + 32 * sp + lane;
+#pragma unroll
+                for (int cb = 0; cb < 4; ++cb) {
+                    float o[kHh], q[kHh];
+                    tmem_ld8(tmem_lane_addr(tmem, sp, kTmemO + kN * cb + h0), o);
+                    tmem_ld8(tmem_lane_addr(tmem, sp, kTmemO + kN * cb + 16 + h0), q);
+                    tmem_wait_ld();
+                    loaded(o); loaded(q);
+#pragma unroll
+                    for (int h = 0; h < kHh; ++h) acc[h * kLora + 128 * cb] = fmaf(q[h], 0.0625f, o[h]);
+                }
+                tc_fence_before();
+                mbar_arrive(&S.o_empty);
+            }
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, kTmemCols);
+    }
+}
+
+cudaError_t k2_kv8_configure() {
+    return cudaFuncSetAttribute(k2_attention_kv8, cudaFuncAttributeMaxDynamicSharedMemorySize, kv8::kSmemBytes);
+}
+
+cudaError_t launch_attention_kv8(const MlaDecodeParams& p, const CUtensorMap& tmap_c, const CUtensorMap& tmap_r,
+                                 float scale_log2, cudaStream_t stream) {
+    const cudaError_t e = launch_pdl(k2_attention_kv8, dim3(p.num_ctas), dim3(kv8::kThreads), kv8::kSmemBytes, stream,
+                                     p, tmap_c, tmap_r, scale_log2);
+    if (e != cudaSuccess) return e;
+    return cudaGetLastError();
+}
+
+}  // namespace mla

@@ -48,6 +48,9 @@
 // the low half of q_c (K1's qa_lo) over the 512 latent columns; kPLo
 // (MLA_FLAG_P_HILO) keeps each probability as bf16 hi + lo in two P buffers, runs
 // the output MMAs on both and sums the row totals over the unrounded values.
+// Window (kWin, MlaDecodeParams.window): the plan's tiles are the half pages that hold a
+// visible row (Visible), and a 32-bit mask of the half page's visible rows takes the
+// place of the count of valid ones, for scores and B fragments alike.
 #include <cuda.h>
 
 #include "mla_common.cuh"
@@ -108,6 +111,17 @@ __device__ __forceinline__ uint32_t mask_pair(uint32_t v, int tok_lo, int valid)
     return v;
 }
 
+// The visible rows of the 32-row half page that starts at row r0, one bit each.
+__device__ __forceinline__ uint32_t seen_rows(const Visible& v, int r0) {
+    auto below = [](int k) -> uint32_t { return k <= 0 ? 0u : (k >= 32 ? ~0u : (1u << k) - 1u); };
+    return below(v.rows - r0) & (below(v.head - r0) | ~below(v.lo - r0));
+}
+// Zero the bf16 halves of a B fragment register whose token's bit is clear.
+__device__ __forceinline__ uint32_t mask_pair_bits(uint32_t v, int tok_lo, uint32_t seen) {
+    const uint32_t b = seen >> tok_lo;
+    return (b & 1 ? v & 0x0000FFFFu : 0u) | (b & 2 ? v & 0xFFFF0000u : 0u);
+}
+
 // Byte offset of (head, 16-byte unit u < 4) in a P block: 64-byte rows whose units
 // are XOR-swizzled with bits 1-2 of the head, so that the 8 rows an ldmatrix
 // reads, and the 8 rows a warp's stores touch, fall in distinct banks.
@@ -115,7 +129,7 @@ __device__ __forceinline__ int p_offset(int head, int u) { return head * 64 + ((
 
 }  // namespace mmak
 
-template <bool kQLo, bool kPLo>
+template <bool kQLo, bool kPLo, bool kWin>
 __global__ void __launch_bounds__(mmak::kThreads, 1)
     k2_attention_mma(const MlaDecodeParams p, const __grid_constant__ CUtensorMap tmap_kv, float scale_log2,
                      int pairs) {
@@ -157,8 +171,15 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
     // The leader's look-ahead over half pages (loads run two half pages ahead).
     TileCursor la{};
     uint32_t issued = 0;
+    // Half page of the request that tile la.index() is.
+    auto half_page = [&]() -> int {
+        if constexpr (kWin)
+            return Visible(p, p.seq_lens[la.b] + new_row_count(p), kHalf).tile(la.index());
+        else
+            return la.index();
+    };
     auto issue_next = [&]() {
-        const int h = la.index();  // half page h of the request: page h / 2, rows 32 (h % 2) ..
+        const int h = half_page();  // half page h of the request: page h / 2, rows 32 (h % 2) ..
         int page = p.block_table[(int64_t)la.b * p.max_blocks + (h >> 1)];
         if (page < 0 || page >= p.n_pages) { record_error(err_sink(p), MLA_DEV_BAD_PAGE); page = 0; }
         const uint32_t slot = issued % kNSlot;
@@ -171,7 +192,7 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
     // Would the half page the leader loads next hold the row K1 appends in this step?
     auto holds_new_row = [&]() -> bool {
         if (!new_row_count(p)) return false;
-        const int row0 = kHalf * la.index(), nr = p.seq_lens[la.b];
+        const int row0 = kHalf * half_page(), nr = p.seq_lens[la.b];
         return nr >= row0 && nr < row0 + kHalf;
     };
     auto init_group = [&]() {
@@ -267,7 +288,8 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
         uint32_t ql[kQLo ? 9 : 1][4];          // kQLo: fragments of the low half of q_c (latent k-steps only)
         float o[16][4];                        // O_w: 16 latent tiles of 8
         float m_run[2], l_run[2];              // heads g, g+8
-        int rows_b = 0;                        // rows attended by the current request
+        int rows_b = 0;                        // rows of the current request
+        Visible vis;                           // kWin: those it sees
         uint32_t i = 0;                        // half pages consumed
         bool ok = true;
         float seg_L[2] = {0.f, 0.f};           // row sums of the last segment, heads g, g+8
@@ -289,6 +311,7 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
         // Row count and Q fragments of request b (the first half page of each segment needs them).
         auto load_query = [&](int b) {
             rows_b = p.seq_lens[b] + new_row_count(p);
+            if constexpr (kWin) vis = Visible(p, rows_b, kHalf);
             const __nv_bfloat16* qrow = qa + (int64_t)b * kQRows * kRow + 144 * w + 2 * t4;
 #pragma unroll
             for (int j = 0; j < 9; ++j) {
@@ -320,6 +343,8 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
             if (first && !q_next) load_query(cur.b);
             q_next = false;
             const int hvalid = min(kHalf, rows_b - kHalf * cur.index());  // valid tokens of this half page
+            uint32_t seen = 0;  // kWin: its visible ones, in place of hvalid
+            if constexpr (kWin) seen = seen_rows(vis, kHalf * vis.tile(cur.index()));
             if (first) {
 #pragma unroll
                 for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -373,10 +398,12 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
                         const float4 x = reinterpret_cast<const float4*>(spart)[(v * 8 + g) * kSRow + 4 * w + t4];
                         lo.x += x.x; lo.y += x.y; hi.x += x.z; hi.y += x.w;
                     }
-                    s[0] = col < hvalid ? lo.x * scale_log2 : -INFINITY;
-                    s[1] = col + 1 < hvalid ? lo.y * scale_log2 : -INFINITY;
-                    s[2] = col < hvalid ? hi.x * scale_log2 : -INFINITY;
-                    s[3] = col + 1 < hvalid ? hi.y * scale_log2 : -INFINITY;
+                    const bool s0 = kWin ? (seen >> col) & 1 : col < hvalid;
+                    const bool s1 = kWin ? (seen >> (col + 1)) & 1 : col + 1 < hvalid;
+                    s[0] = s0 ? lo.x * scale_log2 : -INFINITY;
+                    s[1] = s1 ? lo.y * scale_log2 : -INFINITY;
+                    s[2] = s0 ? hi.x * scale_log2 : -INFINITY;
+                    s[3] = s1 ? hi.y * scale_log2 : -INFINITY;
                 }
                 // ---- probabilities (bf16) for this warp's 8 tokens -> P buffer ----
                 uint8_t* pb = p_s + (i & 1) * kPBytes;
@@ -459,7 +486,15 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
                         const int unit = 2 * (pp & 3) + (m8 >> 1);
                         uint32_t b00, b01, b10, b11;
                         ldsm_x4_t(tbase + chunk * kChunkBytes + tok * 128 + ((unit ^ r8) << 4), b00, b01, b10, b11);
-                        if (hvalid < kHalf) {
+                        if constexpr (kWin) {
+                            if (seen != ~0u) {
+                                const int tl = 16 * ks + 2 * t4;
+                                b00 = mask_pair_bits(b00, tl, seen);
+                                b10 = mask_pair_bits(b10, tl, seen);
+                                b01 = mask_pair_bits(b01, tl + 8, seen);
+                                b11 = mask_pair_bits(b11, tl + 8, seen);
+                            }
+                        } else if (hvalid < kHalf) {
                             const int tl = 16 * ks + 2 * t4;
                             b00 = mask_pair(b00, tl, hvalid);
                             b10 = mask_pair(b10, tl, hvalid);
@@ -558,19 +593,26 @@ __global__ void __launch_bounds__(mmak::kThreads, 1)
 
 int k2_mma_smem_bytes() { return mmak::kSmemBytes; }
 
+namespace {
+using K2Kernel = void (*)(MlaDecodeParams, CUtensorMap, float, int);
+template <bool kWin>
+K2Kernel k2_kernel(bool qlo, bool plo) {
+    return qlo ? (plo ? k2_attention_mma<true, true, kWin> : k2_attention_mma<true, false, kWin>)
+               : (plo ? k2_attention_mma<false, true, kWin> : k2_attention_mma<false, false, kWin>);
+}
+K2Kernel k2_kernel(bool qlo, bool plo, bool win) {
+    return win ? k2_kernel<true>(qlo, plo) : k2_kernel<false>(qlo, plo);
+}
+}  // namespace
+
 cudaError_t k2_mma_configure() {
-    cudaError_t e = cudaFuncSetAttribute(k2_attention_mma<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         mmak::smem_bytes(false));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(k2_attention_mma<true, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 mmak::smem_bytes(false));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(k2_attention_mma<false, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 mmak::smem_bytes(true));
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(k2_attention_mma<true, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 mmak::smem_bytes(true));
-    return e;
+    for (int f = 0; f < 8; ++f) {
+        const bool plo = f & 2;
+        const cudaError_t e = cudaFuncSetAttribute(k2_kernel(f & 1, plo, f & 4),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize, mmak::smem_bytes(plo));
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
 }
 
 cudaError_t launch_attention_mma(const MlaDecodeParams& p, const CUtensorMap& tmap_kv, float scale_log2,
@@ -578,10 +620,9 @@ cudaError_t launch_attention_mma(const MlaDecodeParams& p, const CUtensorMap& tm
     static_assert(mmak::kGroups == 2, "k2_grid assumes two plan CTAs per CTA");
     const int grid = k2_grid(p.num_ctas, sm_count);
     const bool qlo = (p.flags & MLA_FLAG_QC_HILO) != 0, plo = (p.flags & MLA_FLAG_P_HILO) != 0;
-    auto kern = qlo ? (plo ? k2_attention_mma<true, true> : k2_attention_mma<true, false>)
-                    : (plo ? k2_attention_mma<false, true> : k2_attention_mma<false, false>);
-    const cudaError_t e = launch_pdl(kern, dim3(grid), dim3(mmak::kThreads), mmak::smem_bytes(plo), stream, p,
-                                     tmap_kv, scale_log2, k2_pairs(p, sm_count) ? 1 : 0);
+    const cudaError_t e = launch_pdl(k2_kernel(qlo, plo, p.window > 0), dim3(grid), dim3(mmak::kThreads),
+                                     mmak::smem_bytes(plo), stream, p, tmap_kv, scale_log2,
+                                     k2_pairs(p, sm_count) ? 1 : 0);
     if (e != cudaSuccess) return e;
     return cudaGetLastError();
 }

@@ -38,7 +38,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 //   part_ml    f32   [slots][16][2]       split partial: running max (log2 domain), sum of exps
 //   part_acc   f32   [slots][16][512]     split partial: unnormalised sum_t p_t * c_t
 //   qkv        bf16  [batch][3648]        q | kv_a, when the step projects x_n itself (K0)
-//   qa_lo      bf16  [batch][16][512]     q_c - bf16(q_c), with MLA_FLAG_QC_HILO
+//   qa_lo      bf16  [batch][16][512]     q_c - bf16(q_c), with MLA_FLAG_QC_HILO or MLA_FLAG_KV8
 // slots = num_ctas + batch: CTA c writes the partial of request b at slot c + b.
 // ---------------------------------------------------------------------------
 struct WsLayout {
@@ -63,7 +63,7 @@ __host__ __device__ inline uint64_t align256(uint64_t x) { return (x + 255) & ~u
 
 // with_qkv: the step projects x_n itself (MlaDecodeParams.x_n set), and q | kv_a
 // of every request live in the workspace as [batch][3648] bf16.
-// with_qlo: MLA_FLAG_QC_HILO, the low half of q_c lives in qa_lo.
+// with_qlo (stores_q_lo): the low half of q_c lives in qa_lo.
 __host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with_qkv = false, bool with_qlo = false) {
     WsLayout w;
     w.slots = num_ctas + batch;
@@ -79,8 +79,14 @@ __host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with
     return w;
 }
 
+// Whether K1 keeps the low half of q_c: the hi/lo form of the default kernel asks for it, and
+// the 8-bit kernel makes its e4m3 pair of q_c from both halves (a pair of the bf16 q_c alone
+// would carry the bf16 rounding, 4x the pair's own).
+__host__ __device__ inline bool stores_q_lo(const MlaDecodeParams& p) {
+    return (p.flags & (MLA_FLAG_QC_HILO | MLA_FLAG_KV8)) != 0;
+}
 __host__ __device__ inline WsLayout ws_layout(const MlaDecodeParams& p) {
-    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, (p.flags & MLA_FLAG_QC_HILO) != 0);
+    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, stores_q_lo(p));
 }
 
 
@@ -101,7 +107,7 @@ inline int k2_grid(int num_ctas, int sm_count) {
 // flag from the host and test G themselves. Only the default (mma) split-KV kernel
 // pairs.
 inline bool k2_pairs(const MlaDecodeParams& p, int sm_count) {
-    return (p.flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05)) == 0 && p.num_ctas % 2 == 0 &&
+    return (p.flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_KV8)) == 0 && p.num_ctas % 2 == 0 &&
            2 * k2_grid(p.num_ctas, sm_count) == p.num_ctas;
 }
 
@@ -162,16 +168,36 @@ __device__ __forceinline__ bool request_ok(const MlaDecodeParams& p, int b) {
 }
 
 // Rows per tile of the split plan: the default split-KV kernel walks 32-row half
-// pages (its TMA box), the CUDA-core and tensor-memory kernels whole 64-row pages.
+// pages (its TMA box), the others whole 64-row pages.
 __host__ __device__ inline int plan_unit_rows(const MlaDecodeParams& p) {
-    return (p.flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05)) ? kPage : kPage / 2;
+    return (p.flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_KV8)) ? kPage : kPage / 2;
 }
+
+// The rows that a query behind `rows` rows (its own the last) sees: [0, head) and
+// [lo, rows), head <= lo; and the plan tiles of `unit` rows that hold one of them:
+// tile i < n_head is tile i of the request, the others follow from first_tail on.
+struct Visible {
+    int rows, head, lo, n_head, first_tail, n;
+    __device__ Visible() {}
+    __device__ __forceinline__ Visible(const MlaDecodeParams& p, int rows_, int unit) {
+        rows = rows_;
+        lo = p.window > 0 && rows > p.window ? rows - p.window : 0;
+        head = min(p.sinks, lo);
+        n_head = (head + unit - 1) / unit;
+        first_tail = max(n_head, lo / unit);
+        n = n_head + (rows + unit - 1) / unit - first_tail;
+    }
+    __device__ __forceinline__ int tile(int i) const { return i < n_head ? i : first_tail + (i - n_head); }
+    __device__ __forceinline__ bool row(int r) const { return r < rows && (r < head || r >= lo); }
+};
 
 // Tiles request b attends in the split plan: 0 for an invalid request (K1's
 // planner records it), so that no kernel reads outside the block table.
 __device__ __forceinline__ int plan_tiles(const MlaDecodeParams& p, int b) {
     const int unit = plan_unit_rows(p);
-    return request_ok(p, b) ? (p.seq_lens[b] + new_row_count(p) + unit - 1) / unit : 0;
+    if (!request_ok(p, b)) return 0;
+    const int rows = p.seq_lens[b] + new_row_count(p);
+    return p.window > 0 ? Visible(p, rows, unit).n : (rows + unit - 1) / unit;
 }
 
 // ---------------------------------------------------------------------------

@@ -3,7 +3,7 @@
 //
 //  * kv_post: RMSNorm of c_new with HF's two bf16 roundings, RoPE of k_pe_new,
 //    bf16 row appended to the request's page (reference_decode.py:231-237,
-//    src/kernels/attention.h:62-90);
+//    src/kernels/attention.h:62-90), rounded to e4m3 on an 8-bit cache;
 //  * q_pe RoPE, bf16-rounded (reference_decode.py:235);
 //  * q-absorb q_c[h] = q_nope[h] @ W_UK[h] with fp32 accumulation
 //    (reference_decode.py:250, attention.h:171-216): per (block of 64 requests,
@@ -11,7 +11,7 @@
 //    [128 x 128] against a 32 KB slice of W_UK[h] staged by one TMA box; q_nope
 //    and W_UK are bf16 already, so the products are exact; q_c is stored bf16 as
 //    an operand of the attention kernel's score contraction (with
-//    MLA_FLAG_QC_HILO also its remainder, as a second bf16 operand);
+//    MLA_FLAG_QC_HILO or on an 8-bit cache also its remainder, as a second bf16 array);
 //  * the split plan: prefix sum of tiles per request (plan_unit_rows: 32-row half
 //    pages for the default split-KV kernel, 64-row pages for the others), consumed by K2/K3.
 //
@@ -24,6 +24,7 @@
 #include <cuda.h>
 
 #include "mla_common.cuh"
+#include "mla_kv8.cuh"
 #include "mla_mma.cuh"
 #include "mla_rowops.cuh"
 
@@ -193,6 +194,15 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
         if (lane == 0) record_error(err_sink(p), MLA_DEV_BAD_PAGE);
         return;
     }
+    if (p.flags & MLA_FLAG_KV8) {  // the same bf16 row, then rounded to e4m3 under its block's scales
+        float c[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) c[k] = __bfloat162float(outc[k]);
+        append_row8(reinterpret_cast<uint8_t*>(p.kv_cache) + (int64_t)r.page * kPage8,
+                    reinterpret_cast<int8_t*>(p.kv_scales) + (int64_t)r.page * kBlocks8 * 2, r.pos % kPage, c,
+                    bf16_round(lo), bf16_round(hi), lane);
+        return;
+    }
     kv_post_store(reinterpret_cast<__nv_bfloat16*>(p.kv_cache) + ((int64_t)r.page * kPage + r.pos % kPage) * kRow,
                   outc, lo, hi, lane);
 }
@@ -311,8 +321,8 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
             }
         }
     }
-    // MLA_FLAG_QC_HILO: the remainder q_c - bf16(q_c), rounded to bf16, into qa_lo
-    __nv_bfloat16* qa_lo = (p.flags & MLA_FLAG_QC_HILO) ? reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa_lo) : nullptr;
+    // stores_q_lo: the remainder q_c - bf16(q_c), rounded to bf16, into qa_lo
+    __nv_bfloat16* qa_lo = stores_q_lo(p) ? reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa_lo) : nullptr;
     auto lo2 = [](float x, float y) { return pack_bf16(x - bf16_round(x), y - bf16_round(y)); };
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {

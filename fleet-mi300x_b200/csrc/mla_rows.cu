@@ -15,6 +15,7 @@
 // MLA_DEV_BAD_PAGE; such rows are skipped. HBM-bound: 1,152 B read and 1,152 B
 // written per row.
 #include "mla_common.cuh"
+#include "mla_kv8.cuh"
 #include "mla_rowops.cuh"
 
 namespace mla {
@@ -69,7 +70,116 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages(const MlaRowsToP
     }
 }
 
+// The same into an 8-bit cache: one CTA per 16-row block that receives rows, two rows
+// per warp held in registers, so that every row is read once; the block's largest
+// magnitudes meet in shared memory, then the rows are rounded and stored. A first block
+// that holds earlier rows of the request keeps the larger of the old and new scales and
+// holds those rows anew. HBM-bound: 1,152 B read and 576 B written per row.
+//
+// Which block: request b owns the slots row_start[b] / 16 + 2 b .. row_start[b + 1] / 16
+// + 2 b + 1, at least as many as the blocks its rows can touch, whatever first_pos is
+// (n rows touch at most (n - 1) / 16 + 2 blocks, and floor(x + n) - floor(x) >= floor(n)); so the grid follows from the
+// totals the host knows, and a slot past a request's last block is idle.
+__device__ __forceinline__ int64_t block_slot(const MlaRowsToPages& r, int b) {
+    return r.row_start[b] / kBlock8 + 2 * (int64_t)b;
+}
+
+template <bool raw>
+__global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages8(const MlaRowsToPages r) {
+    static_assert(kRowsPerCta * 2 == kBlock8, "two rows per warp");
+    __shared__ float red[kRowsPerCta][2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t v = blockIdx.x;
+    // the request of this slot: largest b with block_slot(b) <= v, 32 probes per round
+    int lo = 0, hi = r.batch;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const uint32_t below = __ballot_sync(0xffffffffu, lane == 0 || (at < hi && block_slot(r, at) <= v));
+        lo += (31 - __clz(below)) * step;
+        hi = min(hi, lo + step);
+    }
+    const int b = lo;
+    const int64_t row0 = r.row_start[b], n = r.row_start[b + 1] - row0;
+    const int64_t first = r.first_pos ? r.first_pos[b] : 0;
+    const int64_t nth = v - block_slot(r, b), blk = (first >> 4) + nth;  // 16-row block of the request, rounded down
+    static_assert(kBlock8 == 16, "shift by 4");
+    if (n <= 0 || nth < 0 || blk > ((first + n - 1) >> 4)) return;
+    // rows [p0, p1) of this block
+    const int64_t limit = min((int64_t)r.max_blocks * kPage, raw ? (int64_t)r.max_pos : INT64_MAX);
+    const int64_t p0 = max(first, blk * kBlock8), p1 = min(first + n, (blk + 1) * kBlock8);
+    const ErrSink err{r.error_word, nullptr};
+    if ((p0 < 0 || p1 > limit) && threadIdx.x == 0) record_error(err, MLA_DEV_BAD_POSITION);
+    if (p0 < 0 || p0 >= limit) return;  // a block is all before position 0 or not at all
+    const int page = r.block_table[(int64_t)b * r.max_blocks + p0 / kPage];
+    if (page < 0 || page >= r.n_pages) {
+        if (threadIdx.x == 0) record_error(err, MLA_DEV_BAD_PAGE);
+        return;
+    }
+    const int slot0 = (int)(blk * kBlock8 % kPage);
+    uint8_t* pg = reinterpret_cast<uint8_t*>(r.kv_cache) + (int64_t)page * kPage8;
+    char2* exps = reinterpret_cast<char2*>(r.kv_scales) + (int64_t)page * kBlocks8 + slot0 / kBlock8;
+
+    float c[2][16], rl[2], rh[2];
+    bool has[2];
+    float ac = 0.f, ar = 0.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int64_t pos = blk * kBlock8 + 2 * warp + k;
+        const int64_t row = row0 + pos - first;  // within the rows given, whatever row_start holds
+        has[k] = pos >= p0 && pos < p1 && pos < limit && row >= 0 && row < r.total_rows;
+        if (!has[k]) continue;
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(r.rows) + row * r.rows_stride;
+        __align__(16) __nv_bfloat16 x[16];
+        if (raw) {
+            kv_post_compute(src, reinterpret_cast<const __nv_bfloat16*>(r.kv_a_norm_w), r.rms_eps,
+                            r.rope_cos + pos * kRope, r.rope_sin + pos * kRope, lane, x, rl[k], rh[k]);
+            rl[k] = bf16_round(rl[k]);
+            rh[k] = bf16_round(rh[k]);
+        } else {
+            reinterpret_cast<uint4*>(x)[0] = reinterpret_cast<const uint4*>(src)[2 * lane];
+            reinterpret_cast<uint4*>(x)[1] = reinterpret_cast<const uint4*>(src)[2 * lane + 1];
+            rl[k] = __bfloat162float(src[kLora + lane]);
+            rh[k] = __bfloat162float(src[kLora + 32 + lane]);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            c[k][j] = __bfloat162float(x[j]);
+            ac = fmaxf(ac, finite_abs(c[k][j]));
+        }
+        ar = fmaxf(ar, fmaxf(finite_abs(rl[k]), finite_abs(rh[k])));
+    }
+    const int before = (int)(p0 - blk * kBlock8);  // earlier rows of the request in this block
+    const char2 old = before ? *exps : make_char2(MLA_SCALE_MIN_EXP, MLA_SCALE_MIN_EXP);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        ac = fmaxf(ac, __shfl_xor_sync(0xffffffffu, ac, o));
+        ar = fmaxf(ar, __shfl_xor_sync(0xffffffffu, ar, o));
+    }
+    if (lane == 0) { red[warp][0] = ac; red[warp][1] = ar; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kRowsPerCta; ++w) { ac = fmaxf(ac, red[w][0]); ar = fmaxf(ar, red[w][1]); }
+    const int e_c = max(scale_exponent(ac), (int)old.x), e_r = max(scale_exponent(ar), (int)old.y);
+    if (before)
+        rescale_rows(pg, slot0 / kBlock8, before, pow2i((int)old.x - e_c), pow2i((int)old.y - e_r), threadIdx.x,
+                     kRowsThreads);
+    if (threadIdx.x == 0) *exps = make_char2((signed char)e_c, (signed char)e_r);
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        if (has[k]) store_row8(pg, slot0 + 2 * warp + k, c[k], rl[k], rh[k], e_c, e_r, lane);
+}
+
 cudaError_t launch_rows_to_pages(const MlaRowsToPages& r, int sm_count, cudaStream_t stream) {
+    if (r.kv_scales) {
+        const int64_t slots = r.total_rows / kBlock8 + 2 * (int64_t)r.batch;
+        if (r.total_rows <= 0) return cudaSuccess;
+        if (slots > INT32_MAX) return cudaErrorInvalidValue;
+        if (r.mode == MLA_ROWS_RAW)
+            k_rows_to_pages8<true><<<(unsigned)slots, kRowsThreads, 0, stream>>>(r);
+        else
+            k_rows_to_pages8<false><<<(unsigned)slots, kRowsThreads, 0, stream>>>(r);
+        return cudaGetLastError();
+    }
     const int64_t need = (r.total_rows + kRowsPerCta - 1) / kRowsPerCta;
     const int64_t cap = (int64_t)sm_count * 16;
     const int grid = (int)(need < cap ? need : cap);

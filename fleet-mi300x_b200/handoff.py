@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import native
-from .attention import _ptr
+from .attention import _ptr, _scales_ptr
 from .cache import PagedLatentCache
 from .native import ROW
 
@@ -28,20 +28,25 @@ ROW_BYTES = ROW * 2
 def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_pos=None, *, raw: bool = False,
                   norm_w: torch.Tensor | None = None, cos: torch.Tensor | None = None,
                   sin: torch.Tensor | None = None, eps: float = 1e-6,
-                  error_word: torch.Tensor | None = None) -> None:
+                  error_word: torch.Tensor | None = None, total: int | None = None) -> None:
     """Write rows[row_start[b]:row_start[b+1]] of request b at positions first_pos[b] + i.
 
     rows: bf16 [total, >= 576] on the cache's device; row_start: [batch + 1] (host or
     device, int); first_pos: [batch] or None (= 0). raw=True takes kv_a rows and needs
     norm_w (kv_a_layernorm weight) and the YaRN tables cos/sin. Does not change seq_lens.
+    On a PagedLatentCache8 the rows are rounded to e4m3 under their blocks' scales.
+    total: row_start's last entry, if the caller knows it; with a device row_start it is
+    otherwise read back, which waits for the device.
     """
     dev = cache.device
     if rows.dtype != torch.bfloat16 or rows.dim() != 2 or rows.shape[1] < ROW or rows.stride(1) != 1:
         raise ValueError("rows must be bf16 [n, >= 576] with contiguous rows")
-    starts = torch.as_tensor(row_start, dtype=torch.int64).to(dev)
+    starts = torch.as_tensor(row_start, dtype=torch.int64)
     if starts.dim() != 1 or starts.numel() != cache.batch + 1:
         raise ValueError(f"row_start needs batch + 1 = {cache.batch + 1} entries")
-    total = int(starts[-1].item())
+    if total is None:
+        total = int(starts[-1].item())
+    starts = starts.to(dev)
     if total > rows.shape[0]:
         raise ValueError(f"row_start ends at {total} but only {rows.shape[0]} rows were given")
     pos = None if first_pos is None else torch.as_tensor(first_pos, dtype=torch.int32).to(dev)
@@ -53,6 +58,7 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     r.row_start, r.first_pos = _ptr(starts), _ptr(pos)
     r.block_table, r.max_blocks, r.n_pages = _ptr(cache.block_table), cache.max_blocks, cache.n_pages
     r.kv_cache = _ptr(cache.pages)
+    r.kv_scales = _scales_ptr(cache)
     if raw:
         if norm_w is None or cos is None or sin is None:
             raise ValueError("raw rows need norm_w, cos and sin")

@@ -13,7 +13,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libmla_decode.so"
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 HEADS, QK_NOPE, QK_ROPE, V_HEAD, KV_LORA, PAGE_SIZE = 16, 128, 64, 128, 512, 64
 ROW = KV_LORA + QK_ROPE
 MAX_BATCH = 65536
@@ -24,6 +24,10 @@ FLAG_NO_NEW_ROW = 0x8
 FLAG_EXCHANGE_SPLIT = 0x10  # peer exchange as K3 + K4 even where the fused K3 applies
 FLAG_QC_HILO = 0x20  # q_c as a bf16 hi/lo pair in the score MMAs (default kernel)
 FLAG_P_HILO = 0x40   # probabilities as a bf16 hi/lo pair in P c_kv, row sums unrounded (default kernel)
+FLAG_KV8 = 0x80      # an 8-bit cache: e4m3 pages, power-of-two scales per 16-row block (MlaDecodeParams.kv_scales)
+PAGE8_BYTES = PAGE_SIZE * ROW  # MLA_PAGE8_BYTES: [64][512] latent, [64][64] rotary e4m3
+SCALE_BLOCK = 16     # MLA_SCALE_BLOCK: rows of a page that share their scales
+SCALE_MIN_EXP = -64  # MLA_SCALE_MIN_EXP
 SHARD_STRIDE = 132
 MAX_PROJECT_BATCH = 64  # MLA_MAX_PROJECT_BATCH: weight-stream projection up to here, tcgen05 GEMM beyond
 STATIC_SCRATCH_BYTES = 32 << 20  # MLA_STATIC_SCRATCH_BYTES, the workspace of mla_decode_step_static
@@ -35,7 +39,7 @@ STATUS = {
     -4: "MLA_E_WORKSPACE", -5: "MLA_E_ARCH", -6: "MLA_E_LAUNCH", -7: "MLA_E_DRIVER", -8: "MLA_E_LIMIT",
 }
 DEV_ERRORS = {0: "ok", 1: "MLA_DEV_BAD_PAGE", 2: "MLA_DEV_BAD_POSITION", 3: "MLA_DEV_TIMEOUT",
-              4: "MLA_DEV_PEER_TIMEOUT"}
+              4: "MLA_DEV_PEER_TIMEOUT", 5: "MLA_DEV_NO_PAGE", 6: "MLA_DEV_BAD_REQUEST"}
 
 EXPORTED = (
     "mla_abi_version", "mla_status_string", "mla_device_error_string", "mla_params_init",
@@ -43,6 +47,8 @@ EXPORTED = (
     "mla_plan_info", "mla_launches_per_step", "mla_combine_shards", "mla_decode_step_static", "mla_project",
     "mla_rows_init", "mla_rows_to_pages", "mla_o_proj", "mla_exchange_bytes", "mla_exchange_alloc",
     "mla_exchange_free", "mla_exchange_open", "mla_exchange_close", "mla_exchange_combine",
+    "mla_pool_init", "mla_pool_scratch_size", "mla_pool_fork", "mla_pool_release", "mla_pool_reserve", "mla_pool_compact",
+    "mla_copy_pages",
 )
 
 
@@ -89,6 +95,7 @@ class MlaDecodeParams(ctypes.Structure):
         ("exchange", ctypes.c_void_p * MAX_RANKS), ("rank", ctypes.c_int32), ("world", ctypes.c_int32),
         ("exchange_batch", ctypes.c_int32), ("exchange_timeout_us", ctypes.c_int32),
         ("error_host", ctypes.c_void_p),
+        ("kv_scales", ctypes.c_void_p), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
     ]
 
 
@@ -107,7 +114,23 @@ class MlaRowsToPages(ctypes.Structure):
         ("kv_cache", ctypes.c_void_p), ("kv_a_norm_w", ctypes.c_void_p),
         ("rope_cos", ctypes.c_void_p), ("rope_sin", ctypes.c_void_p),
         ("max_pos", ctypes.c_int32), ("rms_eps", ctypes.c_float),
-        ("error_word", ctypes.c_void_p),
+        ("error_word", ctypes.c_void_p), ("kv_scales", ctypes.c_void_p),
+    ]
+
+
+MAX_LAYERS = 64  # MLA_MAX_LAYERS
+
+
+class MlaPagePool(ctypes.Structure):
+    """Mirror of MlaPagePool (include/mla_decode.h), field for field."""
+    _fields_ = [
+        ("struct_size", ctypes.c_uint32), ("abi_version", ctypes.c_uint32),
+        ("n_layers", ctypes.c_int32), ("kv8", ctypes.c_int32), ("n_pages", ctypes.c_int32),
+        ("batch", ctypes.c_int32), ("max_blocks", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("pages", ctypes.c_void_p * MAX_LAYERS), ("scales", ctypes.c_void_p * MAX_LAYERS),
+        ("block_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("held", ctypes.c_void_p),
+        ("refs", ctypes.c_void_p), ("scratch", ctypes.c_void_p), ("scratch_bytes", ctypes.c_uint64),
+        ("error_word", ctypes.c_void_p), ("error_host", ctypes.c_void_p),
     ]
 
 
@@ -148,6 +171,15 @@ def load_library(path: Path | str | None = None) -> ctypes.CDLL:
         lib.mla_rows_init.argtypes = [R]
         lib.mla_rows_to_pages.restype = ctypes.c_int
         lib.mla_rows_to_pages.argtypes = [R, ctypes.c_void_p]
+        G, I, V = ctypes.POINTER(MlaPagePool), ctypes.c_int32, ctypes.c_void_p
+        lib.mla_pool_init.restype = None
+        lib.mla_pool_init.argtypes = [G]
+        for fn, args in (("mla_pool_scratch_size", [G, ctypes.POINTER(ctypes.c_uint64)]),
+                         ("mla_pool_fork", [G, V, V, I, V]), ("mla_pool_release", [G, V, I, V]),
+                         ("mla_pool_reserve", [G, V, I, I, V]), ("mla_pool_compact", [G, V]),
+                         ("mla_copy_pages", [G, G, V, V, I, V])):
+            getattr(lib, fn).restype = ctypes.c_int
+            getattr(lib, fn).argtypes = args
         lib.mla_exchange_bytes.restype = ctypes.c_int
         lib.mla_exchange_bytes.argtypes = [ctypes.c_int32, ctypes.c_int32, ctypes.POINTER(ctypes.c_uint64)]
         lib.mla_exchange_alloc.restype = ctypes.c_int
@@ -178,6 +210,12 @@ def new_rows() -> MlaRowsToPages:
     r = MlaRowsToPages()
     load_library().mla_rows_init(ctypes.byref(r))
     return r
+
+
+def new_pool() -> MlaPagePool:
+    p = MlaPagePool()
+    load_library().mla_pool_init(ctypes.byref(p))
+    return p
 
 
 def new_params() -> MlaDecodeParams:

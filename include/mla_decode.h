@@ -26,7 +26,8 @@
  *   kv_b         bf16 [16*256][512]          kv_b_proj.weight: head h rows [256h,256h+128) = W_UK,
  *                                            [256h+128, 256h+256) = W_UV (reference_decode.py:242-248)
  *   rope_cos/sin f32  [max_pos][64]          YaRN tables (reference_decode.py:102-117)
- *   kv_cache     bf16 [n_pages][64][576]     paged latent cache: row = c_kv(512) | k_pe(64)
+ *   kv_cache     bf16 [n_pages][64][576]     paged latent cache: row = c_kv(512) | k_pe(64); or, with
+ *                                            MLA_FLAG_KV8, e4m3 [n_pages][64][512 | 64] (see there)
  *   block_table  i32  [batch][max_blocks]    page ids of each request's logical pages
  *   seq_lens     i32  [batch]                rows cached before this step = position of the new token
  *   out          bf16 [batch][out_stride]    R(out): head h at [128h, 128h+128)
@@ -46,7 +47,7 @@
 extern "C" {
 #endif
 
-#define MLA_ABI_VERSION 6
+#define MLA_ABI_VERSION 7
 
 /* Fixed model dimensions. The reference's launcher refuses any other shape
  * (src/host/fleet_launch.hip:573-577: kv_lora != 512 or qk_rope != 64);
@@ -90,6 +91,8 @@ typedef enum {
 #define MLA_DEV_TIMEOUT 3       /* a bounded on-chip wait gave up (pipeline stall) */
 #define MLA_DEV_PEER_TIMEOUT 4  /* the exchange combine gave up waiting for a shard's flag
                                    (a peer that did not run its step within exchange_timeout_us) */
+#define MLA_DEV_NO_PAGE 5       /* a page pool has too few free pages for the call: nothing was changed */
+#define MLA_DEV_BAD_REQUEST 6   /* a request number outside the batch, or a destination named twice */
 
 /* Flags. */
 #define MLA_FLAG_CHECK_KERNEL 0x2 /* run the CUDA-core split-KV kernel instead of the tensor-core one
@@ -107,9 +110,23 @@ typedef enum {
  * or MLA_FLAG_TCGEN05). Each costs tensor-core issue in K2, not HBM bytes. */
 #define MLA_FLAG_QC_HILO 0x20  /* the absorbed query q_c = q_nope W_UK as a bf16 hi/lo pair: K1 writes both halves,
                                   K2 runs the score MMAs of the 512 latent columns on both (about 16 mantissa bits
-                                  of the fp32 q_c instead of 8); the workspace grows by batch x 16 KB */
+                                  of the fp32 q_c instead of 8); the workspace grows by batch x 16 KB (with MLA_FLAG_KV8 too) */
 #define MLA_FLAG_P_HILO 0x40   /* the probabilities of P c_kv as a bf16 hi/lo pair (two MMAs per step) and the row
                                   sums over the unrounded fp32 values, instead of bf16-rounded probabilities */
+
+/* An 8-bit cache (ABI v7). A page is MLA_PAGE8_BYTES: the latent part [64][512], then the rotary part
+ * [64][64], both e4m3. Every block of MLA_SCALE_BLOCK rows of a page has one power-of-two scale per
+ * part, held as its exponent in kv_scales: value = e4m3 * 2^exponent, where the exponent is the smallest
+ * one, at least MLA_SCALE_MIN_EXP, that brings the block's largest finite magnitude to at most 448 (powers of two, so
+ * that storing a row and re-expressing a block are exact up to e4m3's own rounding). A row that
+ * joins a block whose scale is too small for it raises the scale, and the block's earlier rows are
+ * held anew under it. Infinities and NaN are held as NaN. Its split-KV kernel keeps the scores and the output in tensor
+ * memory (tcgen05.mma kind::f8f6f4): the absorbed query and the probabilities enter as pairs of e4m3
+ * values, together about as precise as bf16. Not with MLA_FLAG_CHECK_KERNEL, _TCGEN05, _QC_HILO, _P_HILO. */
+#define MLA_FLAG_KV8 0x80
+#define MLA_SCALE_BLOCK 16
+#define MLA_SCALE_MIN_EXP (-64)
+#define MLA_PAGE8_BYTES (MLA_PAGE_SIZE * MLA_ROW)
 
 typedef struct MlaDecodeParams {
     uint32_t struct_size; /* sizeof(MlaDecodeParams) */
@@ -139,8 +156,8 @@ typedef struct MlaDecodeParams {
     void* workspace;          /* device scratch, >= mla_workspace_size() bytes, 256-byte aligned */
     uint64_t workspace_bytes;
     int32_t* error_word;      /* optional device int32 (0 = no error); may be NULL */
-    int32_t num_ctas;         /* CTAs of the split plan; 0 = the default: two per SM (the default
-                                 kernel runs two plan CTAs per CTA), one per SM with MLA_FLAG_TCGEN05 */
+    int32_t num_ctas;         /* CTAs of the split plan; 0 = the default: two per SM (the default kernel runs
+                                 two plan CTAs per CTA), one per SM with MLA_FLAG_TCGEN05 or MLA_FLAG_KV8 */
     int32_t flags;            /* MLA_FLAG_* */
 
     /* Sequence-sharded decode (one long sequence split over GPUs by KV range). */
@@ -205,6 +222,14 @@ typedef struct MlaDecodeParams {
      * MLA_E_INVALID_ARG. The reference's host polls its abort word the same way
      * (fleet_runtime.h:194-198, read back by fleet_launch.hip:284-311). */
     int32_t* error_host;
+
+    /* ABI v7. */
+    void* kv_scales;  /* MLA_FLAG_KV8: int8 [n_pages][4][2], the exponents of each 16-row block of a page
+                         (latent part, rotary part), 8-byte aligned; else NULL */
+    int32_t window;   /* sliding window: the query sees the last `window` rows, its own among them; 0 = all.
+                         Only the pages that hold a visible row are read. Default and MLA_FLAG_KV8 kernels;
+                         not with a sequence-sharded step (MLA_FLAG_NO_NEW_ROW, shard_out, world). */
+    int32_t sinks;    /* with window: the first `sinks` rows of a request stay visible; 0 = none */
 } MlaDecodeParams;
 
 #define MLA_SHARD_STRIDE (MLA_V_HEAD + 4)
@@ -309,19 +334,72 @@ typedef struct MlaRowsToPages {
     const int32_t* block_table;
     int32_t max_blocks;
     int32_t n_pages;
-    void* kv_cache;            /* [n_pages][64][576] bf16, 16-byte aligned */
+    void* kv_cache;            /* [n_pages][64][576] bf16, 16-byte aligned; 8-bit pages with kv_scales */
     const void* kv_a_norm_w;   /* MLA_ROWS_RAW: bf16 [512] kv_a_layernorm.weight */
     const float* rope_cos;     /* MLA_ROWS_RAW: [max_pos][64] YaRN tables */
     const float* rope_sin;
     int32_t max_pos;           /* MLA_ROWS_RAW */
     float rms_eps;             /* MLA_ROWS_RAW */
     int32_t* error_word;       /* optional: MLA_DEV_BAD_POSITION / MLA_DEV_BAD_PAGE; such rows are skipped */
+    void* kv_scales;           /* an 8-bit cache (MLA_FLAG_KV8): its exponents, 8-byte aligned; NULL = a bf16 cache */
 } MlaRowsToPages;
 
 /* Fill an MlaRowsToPages with its size and version, everything else zero. */
 void mla_rows_init(MlaRowsToPages* r);
 
 int mla_rows_to_pages(const MlaRowsToPages* r, void* stream);
+
+/* The life of cache pages (ABI v7): fork, release, reserve, compact and copy, for the caches of
+ * all layers of a model in one call (the layers share block_table and seq_lens). The reference keeps
+ * one flat cache per request and has no counterpart. All state is device memory and all calls
+ * are stream-ordered without a host synchronisation, so they may stand in a decode loop or a captured
+ * graph between steps. Pages are taken lowest number first; the outcome depends on the state and
+ * the arguments alone. A page that two requests share must not be appended to: a fork shares full
+ * pages only. src / dst / requests are device int32 arrays. */
+#define MLA_MAX_LAYERS 64
+typedef struct MlaPagePool {
+    uint32_t struct_size;   /* sizeof(MlaPagePool) */
+    uint32_t abi_version;   /* MLA_ABI_VERSION */
+    int32_t n_layers;       /* 1..MLA_MAX_LAYERS */
+    int32_t kv8;            /* 1: 8-bit pages (MLA_FLAG_KV8) with scales; 0: bf16 pages */
+    int32_t n_pages;        /* pages of every layer's pool */
+    int32_t batch;          /* requests: rows of block_table */
+    int32_t max_blocks;     /* row stride of block_table */
+    int32_t reserved;
+    void* pages[MLA_MAX_LAYERS];   /* each layer's kv_cache, 16-byte aligned */
+    void* scales[MLA_MAX_LAYERS];  /* kv8: each layer's kv_scales, 8-byte aligned */
+    int32_t* block_table;   /* [batch][max_blocks] */
+    int32_t* seq_lens;      /* [batch] rows of each request */
+    int32_t* held;          /* [batch] pages of each request: its first `held` block-table entries */
+    int32_t* refs;          /* [n_pages] entries that hold each page; 0 = free; 16-byte aligned */
+    void* scratch;          /* >= mla_pool_scratch_size() bytes, 256-byte aligned; one call at a time */
+    uint64_t scratch_bytes;
+    int32_t* error_word;    /* optional device int32, as in MlaDecodeParams */
+    int32_t* error_host;    /* optional pinned host int32, as in MlaDecodeParams */
+} MlaPagePool;
+
+void mla_pool_init(MlaPagePool* p);
+int mla_pool_scratch_size(const MlaPagePool* p, uint64_t* bytes);
+
+/* For every pair i < n at once: request dst[i] lets go of its pages and becomes a copy of src[i] as it was
+ * before the call: the full pages are shared, the rows of a last page that is not full are copied
+ * into a free page. src[i] == dst[i] changes nothing; a request may be source of some pairs and
+ * destination of another (beams reordered among themselves). The free pages are those before the call.
+ * Too few: MLA_DEV_NO_PAGE and no change. A destination named twice takes its last pair. */
+int mla_pool_fork(const MlaPagePool* p, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
+/* The requests' pages lose a holder each; held = seq_lens = 0. */
+int mla_pool_release(const MlaPagePool* p, const int32_t* requests, int32_t n, void* stream);
+/* Free pages for every request that holds too few for seq_lens + tokens rows (requests = NULL: all of
+ * the batch, n ignored). Too few in all: MLA_DEV_NO_PAGE and no change. */
+int mla_pool_reserve(const MlaPagePool* p, const int32_t* requests, int32_t n, int32_t tokens, void* stream);
+/* Moves held pages to the lowest numbers (with L pages held, those from L on move, in order, to the free ones
+ * before L), block-table entries and counts with them. */
+int mla_pool_compact(const MlaPagePool* p, void* stream);
+/* Page src[i] of every layer of `from` into page dst[i] of `to` (the same layers and kind; they may be
+ * one pool). No page may be named twice in dst, or in both lists of one pool. Uses pages, scales, n_layers, kv8, n_pages and the error
+ * words of `to`; the other fields are not looked at. */
+int mla_copy_pages(const MlaPagePool* to, const MlaPagePool* from, const int32_t* src, const int32_t* dst, int32_t n,
+                   void* stream);
 
 /* Size of the workspace that mla_decode_step_static keeps inside the library, per
  * device: 32 MiB, which holds mla_workspace_size() for up to 463 requests at the
