@@ -59,6 +59,16 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _raw_stream(device: torch.device) -> int:
+    """The current stream of a device as the C ABI takes it (without building a torch.cuda.Stream)."""
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if device.index is None else device.index)
+
+
+def host_word(t: torch.Tensor) -> ctypes.c_int32:
+    """A pinned int32 tensor's first element, read without a torch call."""
+    return ctypes.c_int32.from_address(t.data_ptr())
+
+
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows of a [B, n] tensor. For B = 1 torch may report any
     stride for the batch dimension (0 for a broadcast view), so use the row length."""
@@ -120,6 +130,10 @@ class MlaDecodeAttention:
         # record one (MlaDecodeParams.error_host), so the host sees a failed step
         # without synchronising, also when the step was replayed from a CUDA graph
         self.error_host = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self._error_host = host_word(self.error_host)
+        self._stages = {"all": self.lib.mla_decode_step, "project": self.lib.mla_project,
+                        "prologue": self.lib.mla_prologue, "attention": self.lib.mla_attention,
+                        "merge": self.lib.mla_merge_uv, "combine": self.lib.mla_exchange_combine}
         self._ws: torch.Tensor | None = None
         self._step_key: tuple | None = None   # attend(): params of the last call, reused for the same tensors
         self._step_p: native.MlaDecodeParams | None = None
@@ -224,23 +238,22 @@ class MlaDecodeAttention:
                 raise ValueError(f"shard_out must be f32 [{q.shape[0]}, 16, {native.SHARD_STRIDE}]")
             out = None
         elif out is None:
-            out = torch.empty(q.shape[0], self.cfg.heads * self.cfg.v_head, dtype=torch.bfloat16,
-                              device=self.device)
-        key = (q.data_ptr(), _row_stride(q), kv_a.data_ptr(), _row_stride(kv_a), cache.pages.data_ptr(),
-               cache.block_table.data_ptr(), cache.seq_lens.data_ptr(), cache.n_pages, cache.max_blocks,
-               q.shape[0], _ptr(out), None if out is None else _row_stride(out), _ptr(rope_pos), _ptr(shard_out),
-               new_row, self.flags, self.num_ctas, self.window, self.sinks, _scales_ptr(cache), self.cos.data_ptr(),
+            out = q.new_empty((q.shape[0], self.cfg.heads * self.cfg.v_head))
+        pages, table = cache.pages, cache.block_table
+        key = (q.data_ptr(), q.stride(0), kv_a.data_ptr(), kv_a.stride(0), q.shape[0], pages.data_ptr(), pages.shape[0],
+               table.data_ptr(), table.shape[1], cache.seq_lens.data_ptr(), _scales_ptr(cache), _ptr(rope_pos),
+               _ptr(shard_out), new_row, self.flags, self.num_ctas, self.window, self.sinks, self.cos.data_ptr(),
                self.cos.shape[0], self.kv_b.data_ptr(), None if exchange is None else exchange.key)
         p = self._step_p
         if key != self._step_key or self._ws is None or p.workspace != self._ws.data_ptr():
             p = self.params(q, kv_a, cache, out, rope_pos=rope_pos, shard_out=shard_out, new_row=new_row,
                             exchange=exchange)
             self._step_key, self._step_p = key, p
-        stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-        fn = {"all": self.lib.mla_decode_step, "prologue": self.lib.mla_prologue,
-              "attention": self.lib.mla_attention, "merge": self.lib.mla_merge_uv,
-              "combine": self.lib.mla_exchange_combine}[stage]
-        native.check(fn(ctypes.byref(p), stream), f"mla {stage}", p)
+        elif out is not None:
+            p.out, p.out_stride = out.data_ptr(), _row_stride(out)
+        code = self._stages[stage](p, _raw_stream(self.device))
+        if code:
+            native.check(code, f"mla {stage}", p)
         self._post_check(check)
         return out if shard_out is None else shard_out
 
@@ -261,10 +274,9 @@ class MlaDecodeAttention:
         if key != self._step_key or self._ws is None or p.workspace != self._ws.data_ptr():
             p = self.params(None, None, cache, out, x_n=x_n)
             self._step_key, self._step_p = key, p
-        stream = ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
-        fn = {"all": self.lib.mla_decode_step, "project": self.lib.mla_project, "prologue": self.lib.mla_prologue,
-              "attention": self.lib.mla_attention, "merge": self.lib.mla_merge_uv}[stage]
-        native.check(fn(ctypes.byref(p), stream), f"mla {stage}", p)
+        code = self._stages[stage](p, _raw_stream(self.device))
+        if code:
+            native.check(code, f"mla {stage}", p)
         self._post_check(check)
         return out
 
@@ -336,7 +348,7 @@ class MlaDecodeAttention:
         has recorded a device error. Reads the pinned host word the kernels store the
         code into; no synchronisation, so a step still running is seen once it has
         stored. Clears both words before raising."""
-        code = int(self.error_host[0])
+        code = self._error_host.value
         if code:
             self.error_host.zero_()
             if not torch.cuda.is_current_stream_capturing():
@@ -344,7 +356,7 @@ class MlaDecodeAttention:
             raise native.MlaError(code, "device (a step since the last check)")
 
     def _pre_check(self, check) -> None:
-        if check and not torch.cuda.is_current_stream_capturing():
+        if check and self._error_host.value and not torch.cuda.is_current_stream_capturing():
             self.raise_pending()
 
     def _post_check(self, check) -> None:

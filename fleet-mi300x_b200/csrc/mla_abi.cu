@@ -543,7 +543,9 @@ int mla_workspace_size(const MlaDecodeParams* p, uint64_t* bytes) {
     int ctas = 0;
     st = resolve_ctas(p, &ctas);
     if (st != MLA_OK) return st;
-    *bytes = ws_layout(p->batch, ctas, p->x_n != nullptr, stores_q_lo(*p)).total;
+    MlaDecodeParams q = *p;
+    q.num_ctas = ctas;
+    *bytes = ws_layout(q).total;
     return MLA_OK;
 }
 
@@ -554,7 +556,7 @@ int mla_plan_info(const MlaDecodeParams* p, int32_t* num_ctas, int32_t* num_slot
     st = resolve_ctas(p, &ctas);
     if (st != MLA_OK) return st;
     if (num_ctas) *num_ctas = ctas;
-    if (num_slots) *num_slots = ws_layout(p->batch, ctas, p->x_n != nullptr, stores_q_lo(*p)).slots;
+    if (num_slots) *num_slots = ws_layout(p->batch, ctas).slots;
     return MLA_OK;
 }
 

@@ -32,12 +32,13 @@
 // a 32-row step with visible ones, are zeroed in the tile (0 times stale NaN bytes
 // would be NaN).
 //
-// Warps (512 threads):
+// Warps (640 threads):
 //   0      TMA producer: lanes 0 and 1 each load one page of the tile and its exponents
 //   1      score MMAs, owns the tensor memory
 //   2      output MMAs
 //   4-11   softmax: one token and eight heads per thread; partials of a finished segment
-//   12-15  the query of the next segment: e4m3 pairs under one scale per part
+//   12-19  the query of the next segment: e4m3 pairs under one scale per part (from K1's
+//          largest magnitudes)
 // The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
 // descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
 // clocks of moving them there, elected it takes the 40 that its operands' shared-memory
@@ -53,7 +54,8 @@ namespace mla {
 
 namespace kv8 {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 640;
+constexpr int kQWarps = 8;                      // query warps: two heads each
 constexpr int kSmWarps = 8;                     // softmax warps: 4 token quarters x 2 halves of the heads
 constexpr int kSmThreads = kSmWarps * 32;
 constexpr int kHh = kHeads / 2;                 // heads of a softmax thread
@@ -83,8 +85,7 @@ struct Smem {
     uint64_t o_empty, teardown[2];
     uint64_t exps[kStages][2];  // a page's 4 x 2 exponents
     float q_scale[2][2];        // [buffer][part]: what the pair was divided by
-    float q_red[4][2];
-    float red[2][4][16];
+    alignas(16) float red[2][4][16];
     float lred[4][16];
     uint32_t tmem_base;
     int abort;
@@ -153,6 +154,15 @@ __device__ __forceinline__ bool step_on(const Visible& v, int index, int pages, 
     if ((ks >> 1) >= pages) return false;
     const int r0 = kPage * v.tile(index + (ks >> 1)) + 32 * (ks & 1);
     return r0 < v.rows && (r0 < v.head || r0 + 32 > v.lo);
+}
+
+// The rest of a bounded wait whose first try failed; once a role gave up, every other wait falls
+// through at once. Out of line: the waits are many, and a CTA's first tile runs from a cold
+// instruction cache.
+__device__ __noinline__ bool slow_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* error_word,
+                                       int32_t* error_host) {
+    if (*abort) return false;
+    return mbar_wait(bar, parity, abort, ErrSink{error_word, error_host});
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -224,23 +234,37 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
     pdl_trigger();
     const int vc = blockIdx.x;
 
-    // The split plan: for up to 64 requests from the step's inputs, before the wait on K1
-    // (the rule K1's planner uses); beyond, K1's plan entry after it.
+    // Set-up, side by side: warp 1 takes the tensor memory, warp 2 makes the barriers, and warp 0
+    // the split plan: for up to 64 requests from the step's inputs, before the wait on K1 (the rule
+    // K1's planner uses); beyond, all read K1's plan entry after it.
     constexpr int kPrePlan = 64;
     __shared__ int32_t pre_cum[kPrePlan + 1];
-    __shared__ int32_t pre_tot[2];
     const bool pre = p.batch <= kPrePlan;
-    const int32_t* cum = reinterpret_cast<const int32_t*>(wsb + ws.tiles_cum);
-    PlanEntry pe{};
-    int G = 0;
-    if (threadIdx.x == 0) {
+    if (warp == 0) {
+        if (pre) {
+            const int b0 = 2 * lane, b1 = b0 + 1;
+            const int n0 = b0 < p.batch ? plan_tiles(p, b0) : 0, n1 = b1 < p.batch ? plan_tiles(p, b1) : 0;
+            int incl = n0 + n1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += t;
+            }
+            pre_cum[b0] = incl - n0 - n1;  // beyond the batch: the total
+            pre_cum[b1] = incl - n1;
+            if (lane == 31) pre_cum[kPrePlan] = incl;
+        }
+    } else if (warp == 1) {
+        tmem_alloc(&S.tmem_base, kTmemCols);
+        tmem_relinquish();
+    } else if (warp == 2 && lane == 0) {
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&S.full[i], 2);
             mbar_init(&S.empty[i][0], 1);
             mbar_init(&S.empty[i][1], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&S.q_full[i], 128);
+            mbar_init(&S.q_full[i], kQWarps * 32);
             mbar_init(&S.q_empty[i], 1 + kSmWarps);
             mbar_init(&S.s_full[i], 1);
             mbar_init(&S.p_full[i], kSmThreads);
@@ -250,28 +274,18 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         mbar_init(&S.o_empty, kSmThreads);
         S.abort = 0;
         fence_mbar_init();
+    } else if (warp == 3 && lane == 0) {
         prefetch_tmap(&tmap_c);
         prefetch_tmap(&tmap_r);
     }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+
+    const int32_t* cum = reinterpret_cast<const int32_t*>(wsb + ws.tiles_cum);
+    PlanEntry pe{};
+    int G;
     if (pre) {
-        int n = 0, incl = 0;
-        if (threadIdx.x < kPrePlan) {
-            n = (int)threadIdx.x < p.batch ? plan_tiles(p, threadIdx.x) : 0;
-            incl = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += t;
-            }
-            if (lane == 31) pre_tot[warp] = incl;
-        }
-        __syncthreads();
-        if (threadIdx.x < kPrePlan) {
-            const int before = warp ? pre_tot[0] : 0;
-            pre_cum[threadIdx.x] = before + incl - n;  // beyond the batch: the total
-            if (threadIdx.x == kPrePlan - 1) pre_cum[kPrePlan] = before + incl;
-        }
-        __syncthreads();
         cum = pre_cum;
         const int64_t U = pre_cum[p.batch];
         G = (int)(U < (int64_t)p.num_ctas ? U : (int64_t)p.num_ctas);
@@ -288,28 +302,20 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             pe.cb1 = pre_cum[lo + 1];
         }
     } else {
-        __syncthreads();  // barriers initialised
         pdl_wait();
         MLA_TL_WAITED(1);
         G = reinterpret_cast<const PlanHeader*>(wsb + ws.plan)->G;
-        pe = reinterpret_cast<const PlanEntry*>(wsb + ws.plan + sizeof(PlanHeader))[vc < G ? vc : 0];
+        pe = reinterpret_cast<const PlanEntry*>(wsb + ws.plan + sizeof(PlanHeader))[vc < p.num_ctas ? vc : 0];
     }
-    if (vc >= G) {  // uniform per CTA: no work, nothing allocated
+    const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem_base, 0);
+    if (vc >= G) {  // uniform per CTA: no work
         if (pre) pdl_wait();
+        if (warp == 1) tmem_dealloc(tmem, kTmemCols);
         return;
     }
-
-    if (warp == 1) { tmem_alloc(&S.tmem_base, kTmemCols); tmem_relinquish(); }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tmem = __shfl_sync(0xffffffffu, S.tmem_base, 0);
     volatile int* abort = &S.abort;
-    // A bounded wait; once a role gave up, every other wait falls through at once.
     auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-        if (mbar_try_wait(bar, parity)) return true;
-        if (*abort) return false;
-        return mbar_wait(bar, parity, abort, err);
+        return mbar_try_wait(bar, parity) || slow_wait(bar, parity, abort, p.error_word, p.error_host);
     };
 
     Walk cur;
@@ -457,76 +463,51 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         }
     } else if (warp >= 12) {
         // ------------------------------------------------------------ queries
-        // Warp a converts heads 4a .. 4a + 3: lane holds 2 units of 8 latent values per
-        // head and one rotary unit (head 4a + lane / 8, unit lane % 8).
+        // Warp a converts heads 2a and 2a + 1: lane holds 2 units of 8 latent values per head
+        // and, lanes 0-15, one rotary unit (head 2a + lane / 8, unit lane % 8).
         if (pre) pdl_wait();
         const int a = warp - 12;
         const __nv_bfloat16* qa = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa);
         const __nv_bfloat16* qa_lo = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa_lo);
-        // 8 values of a bf16 unit, plus its remainders
-        auto unit = [](const uint4& v, float (&x)[8]) {
+        const float* qa_max = reinterpret_cast<const float*>(wsb + ws.qa_max);
+        // 8 values, plus their remainders r if any, as e4m3 pairs under the factor f
+        auto put8 = [](const uint4& v, const uint4* r, float f, uint8_t* hi, uint8_t* lo) {
             const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+            uint32_t x[4], y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { x[2 * i] = __low2float(h[i]); x[2 * i + 1] = __high2float(h[i]); }
-        };
-        auto sum = [&](const uint4& v, const uint4& r, float (&x)[8]) {
-            float y[8];
-            unit(v, x);
-            unit(r, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] += y[i];
-        };
-        auto amax8 = [](const float (&x)[8], float m) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, finite_abs(x[i]));
-            return m;
-        };
-        auto put8 = [](const float (&x)[8], float f, uint8_t* hi, uint8_t* lo) {
-            uint32_t wh[2], wl[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t a2[2], b2[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const float u = nan_if_inf(x[4 * i + 2 * k]) * f, w = nan_if_inf(x[4 * i + 2 * k + 1]) * f;
-                    a2[k] = e4m3x2(u, w);
-                    const float2 r = from_e4m3x2(a2[k]);
-                    b2[k] = e4m3x2((u - r.x) * 16.f, (w - r.y) * 16.f);
+            for (int i = 0; i < 4; ++i) {
+                float u = __low2float(h[i]), w = __high2float(h[i]);
+                if (r) {
+                    const __nv_bfloat162 l = reinterpret_cast<const __nv_bfloat162*>(r)[i];
+                    u += __low2float(l);
+                    w += __high2float(l);
                 }
-                wh[i] = a2[0] | (a2[1] << 16);
-                wl[i] = b2[0] | (b2[1] << 16);
+                u = nan_if_inf(u) * f;
+                w = nan_if_inf(w) * f;
+                x[i] = e4m3x2(u, w);
+                const float2 b = from_e4m3x2(x[i]);
+                y[i] = e4m3x2((u - b.x) * 16.f, (w - b.y) * 16.f);
             }
-            *reinterpret_cast<uint2*>(hi) = make_uint2(wh[0], wh[1]);
-            *reinterpret_cast<uint2*>(lo) = make_uint2(wl[0], wl[1]);
+            *reinterpret_cast<uint2*>(hi) = make_uint2(x[0] | (x[1] << 16), x[2] | (x[3] << 16));
+            *reinterpret_cast<uint2*>(lo) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
         };
         for (; cur.valid(); cur.next_request()) {
             const int qb = cur.seg & 1;
             const __nv_bfloat16* q = qa + (int64_t)cur.b * kQRows * kRow;
             const __nv_bfloat16* ql = qa_lo + (int64_t)cur.b * kQRows * kLora;
-            uint4 vc4[8], vl4[8];
+            const float* qm = qa_max + (int64_t)cur.b * kQMax;
+            const float4 m0 = reinterpret_cast<const float4*>(qm)[lane], m1 = reinterpret_cast<const float4*>(qm)[32 + lane];
+            const float mr = qm[kQMaxC];
+            uint4 vh[4], vl[4], vr;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                vc4[i] = reinterpret_cast<const uint4*>(q + (4 * a + (i >> 1)) * kRow)[32 * (i & 1) + lane];
-                vl4[i] = reinterpret_cast<const uint4*>(ql + (4 * a + (i >> 1)) * kLora)[32 * (i & 1) + lane];
+            for (int i = 0; i < 4; ++i) {
+                vh[i] = reinterpret_cast<const uint4*>(q + (2 * a + (i >> 1)) * kRow)[32 * (i & 1) + lane];
+                vl[i] = reinterpret_cast<const uint4*>(ql + (2 * a + (i >> 1)) * kLora)[32 * (i & 1) + lane];
             }
-            float xr[8], x[8];
-            unit(reinterpret_cast<const uint4*>(q + (4 * a + (lane >> 3)) * kRow + kLora)[lane & 7], xr);
-            float mc = 0.f, mr = amax8(xr, 0.f);
+            vr = reinterpret_cast<const uint4*>(q + (2 * a + ((lane >> 3) & 1)) * kRow + kLora)[lane & 7];
+            float mc = fmaxf(fmaxf(fmaxf(m0.x, m0.y), fmaxf(m0.z, m0.w)), fmaxf(fmaxf(m1.x, m1.y), fmaxf(m1.z, m1.w)));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                sum(vc4[i], vl4[i], x);
-                mc = amax8(x, mc);
-            }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, o));
-                mr = fmaxf(mr, __shfl_xor_sync(0xffffffffu, mr, o));
-            }
-            if (lane == 0) { S.q_red[a][0] = mc; S.q_red[a][1] = mr; }
-            named_bar_sync(2, 128);
-            mc = fmaxf(fmaxf(S.q_red[0][0], S.q_red[1][0]), fmaxf(S.q_red[2][0], S.q_red[3][0]));
-            mr = fmaxf(fmaxf(S.q_red[0][1], S.q_red[1][1]), fmaxf(S.q_red[2][1], S.q_red[3][1]));
-            named_bar_sync(2, 128);  // read before the next segment's values
+            for (int o = 16; o; o >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, o));
             const int ec = scale_exponent(mc), er = scale_exponent(mr);
             if (cur.seg >= 2) wait(&S.q_empty[qb], ((cur.seg >> 1) - 1) & 1);
             if (a == 0 && lane == 0) { S.q_scale[qb][0] = pow2i(ec); S.q_scale[qb][1] = pow2i(er); }
@@ -534,16 +515,15 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             uint8_t* qc = smem + kOffQC + qb * kQC;
             uint8_t* qr = smem + kOffQR + qb * kQR;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int n = 4 * a + (i >> 1), col = 8 * (32 * (i & 1) + lane);  // latent column
+            for (int i = 0; i < 4; ++i) {
+                const int n = 2 * a + (i >> 1), col = 8 * (32 * (i & 1) + lane);  // latent column
                 uint8_t* at = qc + (col >> 7) * (kN * 128) + n * 128 + (((((col & 127) >> 4)) ^ (n & 7)) << 4) + (col & 15);
-                sum(vc4[i], vl4[i], x);
-                put8(x, fc, at, at + kHeads * 128);  // row n + 16 has the same swizzle
+                put8(vh[i], &vl[i], fc, at, at + kHeads * 128);  // row n + 16 has the same swizzle
             }
-            {
-                const int n = 4 * a + (lane >> 3), col = 8 * (lane & 7);
+            if (lane < 16) {
+                const int n = 2 * a + (lane >> 3), col = 8 * (lane & 7);
                 uint8_t* at = qr + n * kRope + (((col >> 4) ^ ((n >> 1) & 3)) << 4) + (col & 15);
-                put8(xr, fr, at, at + kHeads * kRope);
+                put8(vr, nullptr, fr, at, at + kHeads * kRope);
             }
             fence_proxy_async_smem();
             mbar_arrive(&S.q_full[qb]);
@@ -608,12 +588,20 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 const float wmax = reduce8<true>(s, lane);
                 if ((lane & 3) == 0) S.red[sb][sp][h0 + (lane >> 2)] = wmax;
                 named_bar_sync(1, kSmThreads);
-                float f[kHh];
+                float f[kHh], t[kHh];
+#pragma unroll
+                for (int k = 0; k < kHh; k += 4) {
+                    float4 x = *reinterpret_cast<const float4*>(&S.red[sb][0][h0 + k]);
+#pragma unroll
+                    for (int w = 1; w < 4; ++w) {
+                        const float4 y = *reinterpret_cast<const float4*>(&S.red[sb][w][h0 + k]);
+                        x = make_float4(fmaxf(x.x, y.x), fmaxf(x.y, y.y), fmaxf(x.z, y.z), fmaxf(x.w, y.w));
+                    }
+                    t[k] = x.x; t[k + 1] = x.y; t[k + 2] = x.z; t[k + 3] = x.w;
+                }
 #pragma unroll
                 for (int h = 0; h < kHh; ++h) {
-                    const float t = fmaxf(fmaxf(S.red[sb][0][h0 + h], S.red[sb][1][h0 + h]),
-                                          fmaxf(S.red[sb][2][h0 + h], S.red[sb][3][h0 + h]));
-                    const float n = fmaxf(m[h], t - 4.f);
+                    const float n = fmaxf(m[h], t[h] - 4.f);
                     f[h] = first ? 1.f : fast_exp2(m[h] - n);
                     m[h] = n;
                     l[h] *= f[h];
@@ -622,7 +610,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     wait(&S.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);
                     tc_fence_after();
                     __syncwarp();
-#pragma unroll
+#pragma unroll 2
                     for (int k = 0; k < 8; ++k) {  // four blocks, hi and lo
                         float o[kHh];
                         const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + 16 * k + h0);

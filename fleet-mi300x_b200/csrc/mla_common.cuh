@@ -39,10 +39,12 @@ constexpr float kLog2e = 1.4426950408889634f;
 //   part_acc   f32   [slots][16][512]     split partial: unnormalised sum_t p_t * c_t
 //   qkv        bf16  [batch][3648]        q | kv_a, when the step projects x_n itself (K0)
 //   qa_lo      bf16  [batch][16][512]     q_c - bf16(q_c), with MLA_FLAG_QC_HILO or MLA_FLAG_KV8
+//   qa_max     f32   [batch][kQMax]       MLA_FLAG_KV8: largest finite |q_c| per 32 columns of a head, then
+//                                         the largest |q_pe| of all heads
 // slots = num_ctas + batch: CTA c writes the partial of request b at slot c + b.
 // ---------------------------------------------------------------------------
 struct WsLayout {
-    uint64_t tiles_cum, plan, qa, part_ml, part_acc, qkv, qa_lo, total;
+    uint64_t tiles_cum, plan, qa, part_ml, part_acc, qkv, qa_lo, qa_max, total;
     int32_t slots;
 };
 
@@ -64,7 +66,10 @@ __host__ __device__ inline uint64_t align256(uint64_t x) { return (x + 255) & ~u
 // with_qkv: the step projects x_n itself (MlaDecodeParams.x_n set), and q | kv_a
 // of every request live in the workspace as [batch][3648] bf16.
 // with_qlo (stores_q_lo): the low half of q_c lives in qa_lo.
-__host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with_qkv = false, bool with_qlo = false) {
+constexpr int kQMaxC = kHeads * (kLora / 32);  // 256
+constexpr int kQMax = kQMaxC + 4;
+__host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with_qkv = false, bool with_qlo = false,
+                                              bool with_qmax = false) {
     WsLayout w;
     w.slots = num_ctas + batch;
     uint64_t off = 0;
@@ -75,6 +80,7 @@ __host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with
     w.part_acc = off;  off = align256(off + uint64_t(w.slots) * kHeads * kLora * 4);
     w.qkv = off;       off = align256(off + (with_qkv ? uint64_t(batch) * kQkvRows * 2 : 0));
     w.qa_lo = off;     off = align256(off + (with_qlo ? uint64_t(batch) * kQRows * kLora * 2 : 0));
+    w.qa_max = off;    off = align256(off + (with_qmax ? uint64_t(batch) * kQMax * 4 : 0));
     w.total = off;
     return w;
 }
@@ -86,7 +92,7 @@ __host__ __device__ inline bool stores_q_lo(const MlaDecodeParams& p) {
     return (p.flags & (MLA_FLAG_QC_HILO | MLA_FLAG_KV8)) != 0;
 }
 __host__ __device__ inline WsLayout ws_layout(const MlaDecodeParams& p) {
-    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, stores_q_lo(p));
+    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, stores_q_lo(p), (p.flags & MLA_FLAG_KV8) != 0);
 }
 
 

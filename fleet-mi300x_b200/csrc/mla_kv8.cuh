@@ -70,18 +70,44 @@ __device__ __forceinline__ void rescale_rows(uint8_t* page, int blk, int n, floa
     }
 }
 
-// One lane's share of a row (16 latent columns 16 lane .., rotary columns lane and 32 + lane)
-// under the exponents e_c, e_r into slot `slot` of a page.
-__device__ __forceinline__ void store_row8(uint8_t* page, int slot, const float (&c)[16], float lo, float hi, int e_c,
-                                           int e_r, int lane) {
+// One lane's share of a bf16 row: 16 latent columns 16 lane .., rotary columns lane and 32 + lane.
+struct RowShare {
+    __nv_bfloat162 c[8];
+    __nv_bfloat16 lo, hi;
+};
+
+// The largest finite magnitudes of a share, into ac and ar; true if it holds an infinity.
+__device__ __forceinline__ bool share_amax(const RowShare& x, float& ac, float& ar) {
+    __nv_bfloat162 m = __habs2(x.c[0]);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) m = __hmax2(m, __habs2(x.c[k]));  // a NaN loses to a number
+    float c = fmaxf(__low2float(m), __high2float(m));
+    float r = fmaxf(fabsf(__bfloat162float(x.lo)), fabsf(__bfloat162float(x.hi)));
+    bool inf = false;
+    if (!(fmaxf(c, r) <= 3.4e38f)) {  // an infinity, or nothing but NaN: look at every value
+        c = 0.f;
+        r = fmaxf(finite_abs(__bfloat162float(x.lo)), finite_abs(__bfloat162float(x.hi)));
+#pragma unroll
+        for (int k = 0; k < 8; ++k) c = fmaxf(c, fmaxf(finite_abs(__low2float(x.c[k])), finite_abs(__high2float(x.c[k]))));
+        inf = true;
+    }
+    ac = fmaxf(ac, c);
+    ar = fmaxf(ar, r);
+    return inf;
+}
+
+// A share under the exponents e_c, e_r into slot `slot` of a page. inf: it may hold an infinity.
+__device__ __forceinline__ void store_share(uint8_t* page, int slot, const RowShare& x, bool inf, int e_c, int e_r,
+                                            int lane) {
     const float f = pow2i(-e_c), g = pow2i(-e_r);
+    auto value = [&](float v) { return inf ? nan_if_inf(v) : v; };
     uint32_t w[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        w[k] = e4m3x4(nan_if_inf(c[4 * k]) * f, nan_if_inf(c[4 * k + 1]) * f, nan_if_inf(c[4 * k + 2]) * f,
-                      nan_if_inf(c[4 * k + 3]) * f);
+        w[k] = e4m3x4(value(__low2float(x.c[2 * k])) * f, value(__high2float(x.c[2 * k])) * f,
+                      value(__low2float(x.c[2 * k + 1])) * f, value(__high2float(x.c[2 * k + 1])) * f);
     *reinterpret_cast<uint4*>(page + slot * kLora + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
-    const uint32_t r = e4m3x2(nan_if_inf(lo) * g, nan_if_inf(hi) * g);
+    const uint32_t r = e4m3x2(value(__bfloat162float(x.lo)) * g, value(__bfloat162float(x.hi)) * g);
     uint8_t* rope = page + kPage8Rope + slot * kRope + lane;
     rope[0] = (uint8_t)r;
     rope[32] = (uint8_t)(r >> 8);
@@ -89,11 +115,9 @@ __device__ __forceinline__ void store_row8(uint8_t* page, int slot, const float 
 
 // One warp appends a row to its slot of a page: the block's scales (exps = its pair of
 // exponents) grow if the row needs it, and the block's earlier rows with them.
-__device__ __forceinline__ void append_row8(uint8_t* page, int8_t* page_exps, int slot, const float (&c)[16], float lo,
-                                            float hi, int lane) {
-    float ac = 0.f, ar = fmaxf(finite_abs(lo), finite_abs(hi));
-#pragma unroll
-    for (int k = 0; k < 16; ++k) ac = fmaxf(ac, finite_abs(c[k]));
+__device__ __forceinline__ void append_row8(uint8_t* page, int8_t* page_exps, int slot, const RowShare& x, int lane) {
+    float ac = 0.f, ar = 0.f;
+    const bool inf = share_amax(x, ac, ar);
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         ac = fmaxf(ac, __shfl_xor_sync(0xffffffffu, ac, o));
@@ -110,7 +134,7 @@ __device__ __forceinline__ void append_row8(uint8_t* page, int8_t* page_exps, in
         __syncwarp();  // every lane has read the exponents
     }
     if (lane == 0) *exps = make_char2((signed char)e_c, (signed char)e_r);
-    store_row8(page, slot, c, lo, hi, e_c, e_r, lane);
+    store_share(page, slot, x, inf, e_c, e_r, lane);
 }
 
 }  // namespace mla

@@ -178,12 +178,20 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
 
     // q_pe of all 16 heads: lane j rotates pair j
     __nv_bfloat16* qrow = qa + (int64_t)b * kQRows * kRow;
+    float qmax = 0.f;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
         float lo, hi;
         rope_pair_r(__low2float(xq[h]), __high2float(xq[h]), r.c0, r.s0, r.c1, r.s1, lo, hi);
         qrow[h * kRow + kLora + lane] = __float2bfloat16_rn(lo);
         qrow[h * kRow + kLora + 32 + lane] = __float2bfloat16_rn(hi);
+        qmax = fmaxf(qmax, fmaxf(finite_abs(bf16_round(lo)), finite_abs(bf16_round(hi))));
+    }
+    if (p.flags & MLA_FLAG_KV8) {  // the largest |q_pe|, for its e4m3 scale
+#pragma unroll
+        for (int o = 16; o; o >>= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
+        if (lane == 0)
+            reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + ws_layout(p).qa_max)[(int64_t)b * kQMax + kQMaxC] = qmax;
     }
     if (!r.append) return;
 
@@ -195,12 +203,14 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
         return;
     }
     if (p.flags & MLA_FLAG_KV8) {  // the same bf16 row, then rounded to e4m3 under its block's scales
-        float c[16];
+        RowShare x;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) c[k] = __bfloat162float(outc[k]);
+        for (int k = 0; k < 8; ++k) x.c[k] = __nv_bfloat162(outc[2 * k], outc[2 * k + 1]);
+        x.lo = __float2bfloat16_rn(lo);
+        x.hi = __float2bfloat16_rn(hi);
         append_row8(reinterpret_cast<uint8_t*>(p.kv_cache) + (int64_t)r.page * kPage8,
-                    reinterpret_cast<int8_t*>(p.kv_scales) + (int64_t)r.page * kBlocks8 * 2, r.pos % kPage, c,
-                    bf16_round(lo), bf16_round(hi), lane);
+                    reinterpret_cast<int8_t*>(p.kv_scales) + (int64_t)r.page * kBlocks8 * 2, r.pos % kPage, x,
+                    lane);
         return;
     }
     kv_post_store(reinterpret_cast<__nv_bfloat16*>(p.kv_cache) + ((int64_t)r.page * kPage + r.pos % kPage) * kRow,
@@ -324,9 +334,29 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
     // stores_q_lo: the remainder q_c - bf16(q_c), rounded to bf16, into qa_lo
     __nv_bfloat16* qa_lo = stores_q_lo(p) ? reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa_lo) : nullptr;
     auto lo2 = [](float x, float y) { return pack_bf16(x - bf16_round(x), y - bf16_round(y)); };
+    // MLA_FLAG_KV8: the largest |q_c| of this warp's 32 columns, per request (the split-KV kernel
+    // then knows its e4m3 scale without a pass over q_c)
+    float* qa_max = (p.flags & MLA_FLAG_KV8) ? reinterpret_cast<float*>(wsb + ws.qa_max) + h * (kLora / 32) + 4 * j + warp
+                                             : nullptr;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
         if (mt >= n_mt) break;
+        if (qa_max) {
+            float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                m0 = fmaxf(m0, fmaxf(finite_abs(acc[mt][n][0]), finite_abs(acc[mt][n][1])));
+                m1 = fmaxf(m1, fmaxf(finite_abs(acc[mt][n][2]), finite_abs(acc[mt][n][3])));
+            }
+#pragma unroll
+            for (int o = 1; o < 4; o <<= 1) {
+                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
+                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
+            }
+            const int r0 = 16 * mt + gq, r1 = r0 + 8;
+            if (t4 == 0 && r0 < nreq) qa_max[(int64_t)(b0 + r0) * kQMax] = m0;
+            if (t4 == 0 && r1 < nreq) qa_max[(int64_t)(b0 + r1) * kQMax] = m1;
+        }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int l = kK1LatQ * j + 32 * warp + 8 * n + 2 * t4;

@@ -85,7 +85,7 @@ __device__ __forceinline__ int64_t block_slot(const MlaRowsToPages& r, int b) {
 }
 
 template <bool raw>
-__global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages8(const MlaRowsToPages r) {
+__global__ void __launch_bounds__(kRowsThreads, raw ? 3 : 5) k_rows_to_pages8(const MlaRowsToPages r) {
     static_assert(kRowsPerCta * 2 == kBlock8, "two rows per warp");
     __shared__ float red[kRowsPerCta][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -110,6 +110,33 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages8(const MlaRowsTo
     const ErrSink err{r.error_word, nullptr};
     if ((p0 < 0 || p1 > limit) && threadIdx.x == 0) record_error(err, MLA_DEV_BAD_POSITION);
     if (p0 < 0 || p0 >= limit) return;  // a block is all before position 0 or not at all
+    // the rows first, so that the block-table entry's latency overlaps theirs
+    RowShare x[2];
+    bool has[2], inf = false;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const int64_t pos = blk * kBlock8 + 2 * warp + k;
+        const int64_t row = row0 + pos - first;  // within the rows given, whatever row_start holds
+        has[k] = pos >= p0 && pos < p1 && pos < limit && row >= 0 && row < r.total_rows;
+        if (!has[k]) continue;
+        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(r.rows) + row * r.rows_stride;
+        if (raw) {
+            __align__(16) __nv_bfloat16 c[16];
+            float lo_f, hi_f;
+            kv_post_compute(src, reinterpret_cast<const __nv_bfloat16*>(r.kv_a_norm_w), r.rms_eps,
+                            r.rope_cos + pos * kRope, r.rope_sin + pos * kRope, lane, c, lo_f, hi_f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[k].c[j] = __nv_bfloat162(c[2 * j], c[2 * j + 1]);
+            x[k].lo = __float2bfloat16_rn(lo_f);
+            x[k].hi = __float2bfloat16_rn(hi_f);
+        } else {
+            uint4* c = reinterpret_cast<uint4*>(x[k].c);
+            c[0] = __ldcs(reinterpret_cast<const uint4*>(src) + 2 * lane);
+            c[1] = __ldcs(reinterpret_cast<const uint4*>(src) + 2 * lane + 1);
+            x[k].lo = src[kLora + lane];
+            x[k].hi = src[kLora + 32 + lane];
+        }
+    }
     const int page = r.block_table[(int64_t)b * r.max_blocks + p0 / kPage];
     if (page < 0 || page >= r.n_pages) {
         if (threadIdx.x == 0) record_error(err, MLA_DEV_BAD_PAGE);
@@ -118,36 +145,10 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages8(const MlaRowsTo
     const int slot0 = (int)(blk * kBlock8 % kPage);
     uint8_t* pg = reinterpret_cast<uint8_t*>(r.kv_cache) + (int64_t)page * kPage8;
     char2* exps = reinterpret_cast<char2*>(r.kv_scales) + (int64_t)page * kBlocks8 + slot0 / kBlock8;
-
-    float c[2][16], rl[2], rh[2];
-    bool has[2];
     float ac = 0.f, ar = 0.f;
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int64_t pos = blk * kBlock8 + 2 * warp + k;
-        const int64_t row = row0 + pos - first;  // within the rows given, whatever row_start holds
-        has[k] = pos >= p0 && pos < p1 && pos < limit && row >= 0 && row < r.total_rows;
-        if (!has[k]) continue;
-        const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(r.rows) + row * r.rows_stride;
-        __align__(16) __nv_bfloat16 x[16];
-        if (raw) {
-            kv_post_compute(src, reinterpret_cast<const __nv_bfloat16*>(r.kv_a_norm_w), r.rms_eps,
-                            r.rope_cos + pos * kRope, r.rope_sin + pos * kRope, lane, x, rl[k], rh[k]);
-            rl[k] = bf16_round(rl[k]);
-            rh[k] = bf16_round(rh[k]);
-        } else {
-            reinterpret_cast<uint4*>(x)[0] = reinterpret_cast<const uint4*>(src)[2 * lane];
-            reinterpret_cast<uint4*>(x)[1] = reinterpret_cast<const uint4*>(src)[2 * lane + 1];
-            rl[k] = __bfloat162float(src[kLora + lane]);
-            rh[k] = __bfloat162float(src[kLora + 32 + lane]);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            c[k][j] = __bfloat162float(x[j]);
-            ac = fmaxf(ac, finite_abs(c[k][j]));
-        }
-        ar = fmaxf(ar, fmaxf(finite_abs(rl[k]), finite_abs(rh[k])));
-    }
+    for (int k = 0; k < 2; ++k)
+        if (has[k]) inf |= share_amax(x[k], ac, ar);
     const int before = (int)(p0 - blk * kBlock8);  // earlier rows of the request in this block
     const char2 old = before ? *exps : make_char2(MLA_SCALE_MIN_EXP, MLA_SCALE_MIN_EXP);
 #pragma unroll
@@ -166,7 +167,7 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages8(const MlaRowsTo
     if (threadIdx.x == 0) *exps = make_char2((signed char)e_c, (signed char)e_r);
 #pragma unroll
     for (int k = 0; k < 2; ++k)
-        if (has[k]) store_row8(pg, slot0 + 2 * warp + k, c[k], rl[k], rh[k], e_c, e_r, lane);
+        if (has[k]) store_share(pg, slot0 + 2 * warp + k, x[k], inf, e_c, e_r, lane);
 }
 
 cudaError_t launch_rows_to_pages(const MlaRowsToPages& r, int sm_count, cudaStream_t stream) {

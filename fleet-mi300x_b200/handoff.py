@@ -18,7 +18,7 @@ import numpy as np
 import torch
 
 from . import native
-from .attention import _ptr, _scales_ptr
+from .attention import _ptr, _raw_stream, _scales_ptr
 from .cache import PagedLatentCache
 from .native import ROW
 
@@ -46,10 +46,11 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
         raise ValueError(f"row_start needs batch + 1 = {cache.batch + 1} entries")
     if total is None:
         total = int(starts[-1].item())
-    starts = starts.to(dev)
+    if starts.device != dev:
+        starts = starts.to(dev)
     if total > rows.shape[0]:
         raise ValueError(f"row_start ends at {total} but only {rows.shape[0]} rows were given")
-    pos = None if first_pos is None else torch.as_tensor(first_pos, dtype=torch.int32).to(dev)
+    pos = None if first_pos is None else torch.as_tensor(first_pos, dtype=torch.int32, device=dev)
     r = native.new_rows()
     r.mode = native.ROWS_RAW if raw else native.ROWS_FINAL
     r.batch = cache.batch
@@ -65,8 +66,7 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
         r.kv_a_norm_w, r.rope_cos, r.rope_sin = _ptr(norm_w), _ptr(cos), _ptr(sin)
         r.max_pos, r.rms_eps = cos.shape[0], eps
     r.error_word = _ptr(error_word)
-    stream = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    native.check(native.load_library().mla_rows_to_pages(ctypes.byref(r), stream), "mla_rows_to_pages")
+    native.check(native.load_library().mla_rows_to_pages(r, _raw_stream(dev)), "mla_rows_to_pages")
 
 
 def read_flat_cache(path: str | Path, layers: int, max_pos: int) -> torch.Tensor:

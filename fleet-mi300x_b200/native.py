@@ -141,6 +141,8 @@ _lock = threading.Lock()
 def load_library(path: Path | str | None = None) -> ctypes.CDLL:
     """Load libmla_decode.so (once) and declare the prototypes."""
     global _lib
+    if _lib is not None and path is None:
+        return _lib
     with _lock:
         if _lib is not None and path is None:
             return _lib

@@ -22,7 +22,7 @@ import ctypes
 import torch
 
 from . import native
-from .attention import _ptr, _scales_ptr
+from .attention import _ptr, _raw_stream, _scales_ptr, host_word
 from .cache import PagedLatentCache, PagedLatentCache8, _check_tensor
 from .native import PAGE_SIZE
 
@@ -50,14 +50,11 @@ def _pages_struct(caches: list[PagedLatentCache]) -> native.MlaPagePool:
 
 
 def _ids(x, device: torch.device) -> torch.Tensor:
-    t = torch.as_tensor(x, dtype=torch.int32, device=device)
+    t = x if isinstance(x, torch.Tensor) and x.dtype == torch.int32 and x.device == device else \
+        torch.as_tensor(x, dtype=torch.int32, device=device)
     if t.dim() != 1 or not t.is_contiguous():
         raise ValueError("request and page numbers must be one contiguous dimension")
     return t
-
-
-def _stream(device: torch.device) -> ctypes.c_void_p:
-    return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
 class PagePool:
@@ -88,6 +85,7 @@ class PagePool:
         self.held, self.refs = held, refs
         self.error_word = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.error_host = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self._error_host = host_word(self.error_host)
         self.lib = native.load_library()
         p = _pages_struct(caches)
         p.batch, p.max_blocks = first.batch, first.max_blocks
@@ -131,9 +129,11 @@ class PagePool:
         return int((self.refs == 0).sum())
 
     def _call(self, name: str, check, *args) -> None:
-        if check and not torch.cuda.is_current_stream_capturing():
+        if check and self._error_host.value and not torch.cuda.is_current_stream_capturing():
             self.raise_pending()
-        native.check(getattr(self.lib, name)(ctypes.byref(self._p), *args, _stream(self.device)), name)
+        code = getattr(self.lib, name)(self._p, *args, _raw_stream(self.device))
+        if code:
+            native.check(code, name)
         if check == "sync" and not torch.cuda.is_current_stream_capturing():
             torch.cuda.current_stream(self.device).synchronize()
             self.raise_pending()
@@ -141,7 +141,7 @@ class PagePool:
     def raise_pending(self) -> None:
         """Raise MlaError if an earlier call recorded a device error (no synchronisation; see
         MlaDecodeAttention.raise_pending). Clears both words before raising."""
-        code = int(self.error_host[0])
+        code = self._error_host.value
         if code:
             self.error_host.zero_()
             if not torch.cuda.is_current_stream_capturing():
@@ -154,13 +154,15 @@ def copy_pages(src_caches, src, dst_caches, dst, *, error_word: torch.Tensor | N
     or lists of layers; the two may be the same): a swap to another pool, or a move within one.
     No destination may appear twice, nor be a source of the same call. Counts and block tables
     are the caller's. A page number outside its pool is skipped and recorded in error_word."""
-    a, b = _layers(src_caches), _layers(dst_caches)
+    a = _layers(src_caches)
+    b = a if dst_caches is src_caches else _layers(dst_caches)
     if len(a) != len(b) or type(a[0]) is not type(b[0]) or a[0].device != b[0].device:
         raise ValueError("copies go between caches of one class, device and number of layers")
     src, dst = _ids(src, a[0].device), _ids(dst, a[0].device)
     if src.numel() != dst.numel():
         raise ValueError(f"{src.numel()} sources for {dst.numel()} destinations")
-    p, q = _pages_struct(a), _pages_struct(b)
+    p = _pages_struct(a)
+    q = p if b is a else _pages_struct(b)
     q.error_word = _ptr(error_word)
-    native.check(native.load_library().mla_copy_pages(ctypes.byref(q), ctypes.byref(p), _ptr(src), _ptr(dst), src.numel(),
-                                                      _stream(a[0].device)), "mla_copy_pages")
+    native.check(native.load_library().mla_copy_pages(q, p, _ptr(src), _ptr(dst), src.numel(),
+                                                      _raw_stream(a[0].device)), "mla_copy_pages")
