@@ -135,6 +135,9 @@ class MlaDecodeAttention:
                         "prologue": self.lib.mla_prologue, "attention": self.lib.mla_attention,
                         "merge": self.lib.mla_merge_uv, "combine": self.lib.mla_exchange_combine}
         self._ws: torch.Tensor | None = None
+        # the column norms of W_UK, from which a step on an 8-bit cache knows its query's scale
+        self.uk_norm = torch.empty(cfg.heads, dtype=torch.float32, device=dev)
+        native.check(self.lib.mla_uk_norms(_ptr(self.kv_b), _ptr(self.uk_norm), _raw_stream(dev)), "mla_uk_norms")
         self._step_key: tuple | None = None   # attend(): params of the last call, reused for the same tensors
         self._step_p: native.MlaDecodeParams | None = None
 
@@ -177,6 +180,7 @@ class MlaDecodeAttention:
         if isinstance(cache, PagedLatentCache8):
             p.flags |= native.FLAG_KV8
             p.kv_scales = _ptr(cache.scales)
+            p.uk_norm = _ptr(self.uk_norm)
         p.window, p.sinks = self.window, self.sinks
         p.rope_pos = _ptr(rope_pos)
         p.shard_out = _ptr(shard_out)

@@ -18,6 +18,7 @@ cudaError_t launch_prologue(const MlaDecodeParams& p, const CUtensorMap& tmap_kv
 cudaError_t launch_attention_tc(const MlaDecodeParams& p, const CUtensorMap& tmap_kv, const CUtensorMap& tmap_q,
                                 float scale_log2, cudaStream_t stream);
 cudaError_t launch_attention_check(const MlaDecodeParams& p, float scale_log2, cudaStream_t stream);
+cudaError_t launch_uk_norms(const void* kv_b, float* norms, cudaStream_t stream);
 cudaError_t launch_merge_uv(const MlaDecodeParams& p, const CUtensorMap& tmap_kvb, int sm_count, bool fused,
                             cudaStream_t stream);
 bool k3_fused_fits(int batch, int sm_count);
@@ -403,7 +404,7 @@ int prepare(const MlaDecodeParams* p, MlaDecodeParams* out) {
     if ((p->flags & (MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO)) && (p->flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05)))
         return MLA_E_INVALID_ARG;  // the hi/lo forms exist in the default kernel only
     const bool kv8 = (p->flags & MLA_FLAG_KV8) != 0;
-    if (kv8 != (p->kv_scales != nullptr)) return MLA_E_INVALID_ARG;
+    if (kv8 != (p->kv_scales != nullptr) || kv8 != (p->uk_norm != nullptr)) return MLA_E_INVALID_ARG;
     if (kv8 && (p->flags & (MLA_FLAG_CHECK_KERNEL | MLA_FLAG_TCGEN05 | MLA_FLAG_QC_HILO | MLA_FLAG_P_HILO)))
         return MLA_E_INVALID_ARG;  // an 8-bit cache has its own split-KV kernel, without these forms
     if (p->window < 0 || p->sinks < 0 || (p->sinks > 0 && p->window == 0)) return MLA_E_INVALID_ARG;
@@ -430,7 +431,7 @@ int prepare(const MlaDecodeParams* p, MlaDecodeParams* out) {
     if (!aligned(p->kv_cache, 16) || !aligned(p->kv_b, 16) || !aligned(p->workspace, 256) ||
         !aligned(p->q, 4) || (p->q_stride & 1) || (p->out_stride & 1) || !aligned(p->kv_a, 2) || !aligned(p->out, 4) || !aligned(p->kv_a_norm_w, 2) ||
         !aligned(p->rope_cos, 4) || !aligned(p->rope_sin, 4) || !aligned(p->rope_pos, 4) ||
-        !aligned(p->shard_out, 16) || !aligned(p->kv_scales, 8))
+        !aligned(p->shard_out, 16) || !aligned(p->kv_scales, 8) || !aligned(p->uk_norm, 4))
         return MLA_E_MISALIGNED;
     int sms = 0;
     st = device_info(&sms);
@@ -601,6 +602,14 @@ int mla_rows_to_pages(const MlaRowsToPages* r, void* stream) {
     const int st = device_info(&sms);
     if (st != MLA_OK) return st;
     return launch_rows_to_pages(*r, sms, (cudaStream_t)stream) == cudaSuccess ? MLA_OK : MLA_E_LAUNCH;
+}
+
+int mla_uk_norms(const void* kv_b, float* norms, void* stream) {
+    if (!kv_b || !norms) return MLA_E_INVALID_ARG;
+    if (!aligned(kv_b, 16) || !aligned(norms, 4)) return MLA_E_MISALIGNED;
+    const int st = device_info(nullptr);
+    if (st != MLA_OK) return st;
+    return launched(launch_uk_norms(kv_b, norms, (cudaStream_t)stream));
 }
 
 void mla_pool_init(MlaPagePool* p) {

@@ -32,13 +32,12 @@
 // a 32-row step with visible ones, are zeroed in the tile (0 times stale NaN bytes
 // would be NaN).
 //
-// Warps (640 threads):
+// Warps (384 threads):
 //   0      TMA producer: lanes 0 and 1 each load one page of the tile and its exponents
 //   1      score MMAs, owns the tensor memory
 //   2      output MMAs
+//   3      loads the query of the next segment: K1 left it as the operand's image
 //   4-11   softmax: one token and eight heads per thread; partials of a finished segment
-//   12-19  the query of the next segment: e4m3 pairs under one scale per part (from K1's
-//          largest magnitudes)
 // The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
 // descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
 // clocks of moving them there, elected it takes the 40 that its operands' shared-memory
@@ -54,8 +53,7 @@ namespace mla {
 
 namespace kv8 {
 
-constexpr int kThreads = 640;
-constexpr int kQWarps = 8;                      // query warps: two heads each
+constexpr int kThreads = 384;
 constexpr int kSmWarps = 8;                     // softmax warps: 4 token quarters x 2 halves of the heads
 constexpr int kSmThreads = kSmWarps * 32;
 constexpr int kHh = kHeads / 2;                 // heads of a softmax thread
@@ -66,16 +64,14 @@ constexpr int kHalfC = kPage * kLora;           // one page's latent bytes in a 
 constexpr int kHalfR = kPage * kRope;
 constexpr int kStageC = 2 * kHalfC;             // 65,536
 constexpr int kStageR = 2 * kHalfR;             // 8,192
-constexpr int kN = 2 * kHeads;                  // hi | lo
-constexpr int kQC = kN * kLora;                 // [4 column blocks][32][128 B]
-constexpr int kQR = kN * kRope;                 // [32][64 B]
+constexpr int kN = kQ8N;                        // hi | lo
+constexpr int kQ = kQ8C + kQ8R;                 // a request's query image
 constexpr int kP = kTok * kN;                   // [128 tokens][32 B]
 
 constexpr int kOffC = 0;
 constexpr int kOffR = kOffC + kStages * kStageC;
-constexpr int kOffQC = kOffR + kStages * kStageR;
-constexpr int kOffQR = kOffQC + 2 * kQC;
-constexpr int kOffP = kOffQR + 2 * kQR;
+constexpr int kOffQ = kOffR + kStages * kStageR;
+constexpr int kOffP = kOffQ + 2 * kQ;
 constexpr int kOffMisc = kOffP + 2 * kP;
 
 struct Smem {
@@ -84,7 +80,7 @@ struct Smem {
     uint64_t s_full[2], p_full[2], pv_done[2];
     uint64_t o_empty, teardown[2];
     uint64_t exps[kStages][2];  // a page's 4 x 2 exponents
-    float q_scale[2][2];        // [buffer][part]: what the pair was divided by
+    alignas(16) float q_scale[2][kQScale];  // [buffer]: per head, then the rotary part's
     alignas(16) float red[2][4][16];
     float lred[4][16];
     uint32_t tmem_base;
@@ -92,7 +88,7 @@ struct Smem {
 };
 constexpr int kSmemBytes = kOffMisc + (int)sizeof(Smem) + 1024;  // + alignment slack
 static_assert(kSmemBytes <= 232448, "K2 (8-bit) shared memory exceeds 227 KB");
-static_assert(kOffP % 1024 == 0 && kOffQR % 1024 == 0, "operands must stay 1024-byte aligned");
+static_assert(kOffP % 1024 == 0 && kOffQ % 1024 == 0 && kQ % 1024 == 0, "operands must stay 1024-byte aligned");
 
 // Tensor memory columns: two score buffers (latent 32 | rotary 32), four output blocks.
 constexpr int kTmemS = 0, kTmemO = 128, kTmemCols = 256;
@@ -191,6 +187,14 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const float (&v)[kHh]) 
                  : "memory");
 }
 
+// An untiled copy global -> shared, completing on an mbarrier (16-byte aligned, a multiple of 16 bytes).
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(smem_dst)),
+                 "l"(src), "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
 // Reduction of 8 values over the 32 lanes of a warp by halving exchanges: lanes 4 h ..
 // 4 h + 3 end with value h.
 template <bool kMax>
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             mbar_init(&S.empty[i][1], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&S.q_full[i], kQWarps * 32);
+            mbar_init(&S.q_full[i], 1);
             mbar_init(&S.q_empty[i], 1 + kSmWarps);
             mbar_init(&S.s_full[i], 1);
             mbar_init(&S.p_full[i], kSmThreads);
@@ -388,8 +392,8 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         // ------------------------------------------------------------ score MMAs
         const uint64_t dc = desc_of(smem_u32(smem + kOffC), kGroup, kSw128);
         const uint64_t dr = desc_of(smem_u32(smem + kOffR), 8 * kRope, kSw64);
-        const uint64_t dqc = desc_of(smem_u32(smem + kOffQC), 1024, kSw128);
-        const uint64_t dqr = desc_of(smem_u32(smem + kOffQR), 8 * kRope, kSw64);
+        const uint64_t dqc = desc_of(smem_u32(smem + kOffQ), 1024, kSw128);
+        const uint64_t dqr = desc_of(smem_u32(smem + kOffQ + kQ8C), 8 * kRope, kSw64);
         uint32_t j = 0;
         for (; cur.valid(); cur.next(), ++j) {
             const uint32_t st = j % kStages, qb = cur.seg & 1, sb = j & 1;
@@ -398,8 +402,8 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             if (j >= 2 && !wait(&S.p_full[sb], ((j - 2) >> 1) & 1)) break;  // the buffer's scores were read
             tc_fence_after();
             __syncwarp();
-            const uint64_t a = dc + ((st * kStageC) >> 4), b = dqc + ((qb * kQC) >> 4);
-            const uint64_t ar = dr + ((st * kStageR) >> 4), br = dqr + ((qb * kQR) >> 4);
+            const uint64_t a = dc + ((st * kStageC) >> 4), b = dqc + ((qb * kQ) >> 4);
+            const uint64_t ar = dr + ((st * kStageR) >> 4), br = dqr + ((qb * kQ) >> 4);
             const uint32_t d = tmem + kTmemS + 64 * sb;
             const bool last = cur.last();
             if (elect_one()) {
@@ -461,72 +465,24 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             tc_commit(&S.teardown[1]);
             mbar_drain(&S.teardown[1], 0, err);
         }
-    } else if (warp >= 12) {
+    } else if (warp == 3) {
         // ------------------------------------------------------------ queries
-        // Warp a converts heads 2a and 2a + 1: lane holds 2 units of 8 latent values per head
-        // and, lanes 0-15, one rotary unit (head 2a + lane / 8, unit lane % 8).
-        if (pre) pdl_wait();
-        const int a = warp - 12;
-        const __nv_bfloat16* qa = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa);
-        const __nv_bfloat16* qa_lo = reinterpret_cast<const __nv_bfloat16*>(wsb + ws.qa_lo);
-        const float* qa_max = reinterpret_cast<const float*>(wsb + ws.qa_max);
-        // 8 values, plus their remainders r if any, as e4m3 pairs under the factor f
-        auto put8 = [](const uint4& v, const uint4* r, float f, uint8_t* hi, uint8_t* lo) {
-            const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
-            uint32_t x[4], y[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float u = __low2float(h[i]), w = __high2float(h[i]);
-                if (r) {
-                    const __nv_bfloat162 l = reinterpret_cast<const __nv_bfloat162*>(r)[i];
-                    u += __low2float(l);
-                    w += __high2float(l);
-                }
-                u = nan_if_inf(u) * f;
-                w = nan_if_inf(w) * f;
-                x[i] = e4m3x2(u, w);
-                const float2 b = from_e4m3x2(x[i]);
-                y[i] = e4m3x2((u - b.x) * 16.f, (w - b.y) * 16.f);
+        if (lane == 0) {
+            if (pre) pdl_wait();
+            const char* img = wsb + ws.qa;
+            const float* q_scale = reinterpret_cast<const float*>(wsb + ws.q_scale);
+            uint32_t issued = 0;
+            for (; cur.valid(); cur.next_request(), ++issued) {
+                const uint32_t qb = cur.seg & 1;
+                if (cur.seg >= 2 && !wait(&S.q_empty[qb], ((cur.seg >> 1) - 1) & 1)) break;
+                mbar_arrive_expect_tx(&S.q_full[qb], kQ + kQScale * 4);
+                bulk_load(smem + kOffQ + qb * kQ, img + (int64_t)cur.b * kQ, kQ, &S.q_full[qb]);
+                bulk_load(S.q_scale[qb], q_scale + (int64_t)cur.b * kQScale, kQScale * 4, &S.q_full[qb]);
             }
-            *reinterpret_cast<uint2*>(hi) = make_uint2(x[0] | (x[1] << 16), x[2] | (x[3] << 16));
-            *reinterpret_cast<uint2*>(lo) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
-        };
-        for (; cur.valid(); cur.next_request()) {
-            const int qb = cur.seg & 1;
-            const __nv_bfloat16* q = qa + (int64_t)cur.b * kQRows * kRow;
-            const __nv_bfloat16* ql = qa_lo + (int64_t)cur.b * kQRows * kLora;
-            const float* qm = qa_max + (int64_t)cur.b * kQMax;
-            const float4 m0 = reinterpret_cast<const float4*>(qm)[lane], m1 = reinterpret_cast<const float4*>(qm)[32 + lane];
-            const float mr = qm[kQMaxC];
-            uint4 vh[4], vl[4], vr;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                vh[i] = reinterpret_cast<const uint4*>(q + (2 * a + (i >> 1)) * kRow)[32 * (i & 1) + lane];
-                vl[i] = reinterpret_cast<const uint4*>(ql + (2 * a + (i >> 1)) * kLora)[32 * (i & 1) + lane];
+            for (uint32_t qb = 0; qb < 2; ++qb) {  // drained as the pages are
+                const uint32_t fills = issued / 2 + (qb < issued % 2 ? 1u : 0u);
+                if (fills) mbar_drain(&S.q_full[qb], (fills - 1) & 1, err);
             }
-            vr = reinterpret_cast<const uint4*>(q + (2 * a + ((lane >> 3) & 1)) * kRow + kLora)[lane & 7];
-            float mc = fmaxf(fmaxf(fmaxf(m0.x, m0.y), fmaxf(m0.z, m0.w)), fmaxf(fmaxf(m1.x, m1.y), fmaxf(m1.z, m1.w)));
-#pragma unroll
-            for (int o = 16; o; o >>= 1) mc = fmaxf(mc, __shfl_xor_sync(0xffffffffu, mc, o));
-            const int ec = scale_exponent(mc), er = scale_exponent(mr);
-            if (cur.seg >= 2) wait(&S.q_empty[qb], ((cur.seg >> 1) - 1) & 1);
-            if (a == 0 && lane == 0) { S.q_scale[qb][0] = pow2i(ec); S.q_scale[qb][1] = pow2i(er); }
-            const float fc = pow2i(-ec), fr = pow2i(-er);
-            uint8_t* qc = smem + kOffQC + qb * kQC;
-            uint8_t* qr = smem + kOffQR + qb * kQR;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int n = 2 * a + (i >> 1), col = 8 * (32 * (i & 1) + lane);  // latent column
-                uint8_t* at = qc + (col >> 7) * (kN * 128) + n * 128 + (((((col & 127) >> 4)) ^ (n & 7)) << 4) + (col & 15);
-                put8(vh[i], &vl[i], fc, at, at + kHeads * 128);  // row n + 16 has the same swizzle
-            }
-            if (lane < 16) {
-                const int n = 2 * a + (lane >> 3), col = 8 * (lane & 7);
-                uint8_t* at = qr + n * kRope + (((col >> 4) ^ ((n >> 1) & 3)) << 4) + (col & 15);
-                put8(vr, nullptr, fr, at, at + kHeads * kRope);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(&S.q_full[qb]);
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax, partials
@@ -534,31 +490,34 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         const int h0 = warp < 8 ? 0 : kHh;  // this thread's heads: h0 .. h0 + 7
         float* part_ml = reinterpret_cast<float*>(wsb + ws.part_ml);
         float* part_acc = reinterpret_cast<float*>(wsb + ws.part_acc);
-        if (pre) pdl_wait();   // the previous step's merge has read the partials
         float m[kHh], l[kHh];  // reference (log2 domain), this thread's part of the row sum
-        float qsc = 0.f, qsr = 0.f;
+        float qs[kHh], qsr = 0.f;  // what this thread's heads' scores are multiplied by, latent and rotary
         Visible vis;
         uint32_t j = 0;
-        for (; cur.valid(); cur.next(), ++j) {
+        // The first pass is a rehearsal without a visible row, while the first tile is on its way: it
+        // fetches the code (measured: 3,000 clocks for a first tile from a cold cache, 1,000 for a later
+        // one). It waits for nothing, signals nothing and stores nothing outside the P buffer.
+        for (bool dry = true; dry || cur.valid();) {
             const uint32_t st = j % kStages, sb = j & 1;
             const bool first = cur.first(), last = cur.last();
             if (first) vis = visible(cur.b);
             const int index = cur.index(), pages = cur.pages();
-            const bool sees = half < pages && vis.row(kPage * vis.tile(index + half) + slot);
-            wait(&S.full[st], (j / kStages) & 1);  // the exponents, and the tile itself where rows are zeroed
+            const bool sees = !dry && half < pages && vis.row(kPage * vis.tile(index + half) + slot);
+            if (!dry) wait(&S.full[st], (j / kStages) & 1);  // the exponents, and the tile itself where rows are zeroed
             const char2 ex = sees ? reinterpret_cast<const char2*>(&S.exps[st][half])[slot / kBlock8] : make_char2(0, 0);
             if (first) {
                 const int qb = cur.seg & 1;
-                wait(&S.q_full[qb], (cur.seg >> 1) & 1);
-                qsc = S.q_scale[qb][0] * scale_log2;
-                qsr = S.q_scale[qb][1] * scale_log2;
+                if (!dry) wait(&S.q_full[qb], (cur.seg >> 1) & 1);
+                qsr = S.q_scale[qb][kHeads] * scale_log2;
+#pragma unroll
+                for (int h = 0; h < kHh; ++h) qs[h] = S.q_scale[qb][h0 + h] * scale_log2;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S.q_empty[qb]);
+                if (!dry && lane == 0) mbar_arrive(&S.q_empty[qb]);
 #pragma unroll
                 for (int h = 0; h < kHh; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
             }
-            const float fc = pow2i(ex.x) * qsc, fr = pow2i(ex.y) * qsr, e = (float)ex.x;
-            wait(&S.s_full[sb], (j >> 1) & 1);
+            const float fc = pow2i(ex.x), fr = pow2i(ex.y) * qsr, e = (float)ex.x;
+            if (!dry) wait(&S.s_full[sb], (j >> 1) & 1);
             tc_fence_after();
             __syncwarp();
             float s[kHh];
@@ -573,7 +532,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 loaded(s); loaded(a); loaded(b); loaded(c);
 #pragma unroll
                 for (int h = 0; h < kHh; ++h)
-                    s[h] = sees ? fmaf(fmaf(a[h], 0.0625f, s[h]), fc, fmaf(fmaf(c[h], 0.0625f, b[h]), fr, e)) : -INFINITY;
+                    s[h] = sees ? fmaf(fmaf(a[h], 0.0625f, s[h]), fc * qs[h], fmaf(fmaf(c[h], 0.0625f, b[h]), fr, e)) : -INFINITY;
             }
             // ---- the reference per head: kept unless a score exceeds it 256-fold (16-fold the
             // largest so far); the first tile of a segment sets it ----
@@ -636,9 +595,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     const float u = sees ? fast_exp2(s[h] - m[h]) : 0.f, w = sees ? fast_exp2(s[h + 1] - m[h + 1]) : 0.f;
                     l[h] = fmaf(u, back, l[h]);
                     l[h + 1] = fmaf(w, back, l[h + 1]);
-                    x[i] = e4m3x2(u, w);
-                    const float2 r = from_e4m3x2(x[i]);
-                    y[i] = e4m3x2((u - r.x) * 16.f, (w - r.y) * 16.f);
+                    e4m3_pairs(u, w, x[i], y[i]);
                 }
                 hi[k] = x[0] | (x[1] << 16);
                 lo[k] = y[0] | (y[1] << 16);
@@ -650,7 +607,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 *reinterpret_cast<uint2*>(pt + (sw << 4)) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(pt + ((sw ^ 1) << 4)) = make_uint2(lo[0], lo[1]);
             }
-            if (!sees && step_on(vis, index, pages, sp)) {  // 0 * stale bytes must be 0
+            if (!sees && !dry && step_on(vis, index, pages, sp)) {  // 0 * stale bytes must be 0
                 uint8_t* row = smem + kOffC + st * kStageC + (tok >> 3) * kGroup + (tok & 7) * 128 + (h0 >> 3) * 2048;
 #pragma unroll 4
                 for (int i = 0; i < kLora / 32; ++i)  // this half's two column blocks
@@ -658,14 +615,14 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             }
             fence_proxy_async_smem();
             tc_fence_before();
-            mbar_arrive(&S.p_full[sb]);
+            if (!dry) mbar_arrive(&S.p_full[sb]);
 
-            if (last) {
+            if (last || dry) {
                 const float ls = reduce8<false>(l, lane);
                 if ((lane & 3) == 0) S.lred[sp][h0 + (lane >> 2)] = ls;
                 named_bar_sync(1, kSmThreads);
                 const int64_t part = (int64_t)vc + cur.b;
-                if (sp == 0 && lane < kHh) {
+                if (sp == 0 && lane < kHh && !dry) {
                     float mh = 0.f;
 #pragma unroll
                     for (int h = 0; h < kHh; ++h) if (h == lane) mh = m[h];
@@ -674,7 +631,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     *reinterpret_cast<float2*>(part_ml + (part * kHeads + h) * 2) = make_float2(mh, lh);
                 }
                 __syncwarp();
-                wait(&S.pv_done[sb], (j >> 1) & 1);
+                if (!dry) wait(&S.pv_done[sb], (j >> 1) & 1);
                 tc_fence_after();
                 __syncwarp();
                 float* acc = part_acc + (part * kHeads + h0) * kLora + 32 * sp + lane;
@@ -686,11 +643,19 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     tmem_wait_ld();
                     loaded(o); loaded(q);
 #pragma unroll
-                    for (int h = 0; h < kHh; ++h) acc[h * kLora + 128 * cb] = fmaf(q[h], 0.0625f, o[h]);
+                    for (int h = 0; h < kHh; ++h)
+                        if (!dry) acc[h * kLora + 128 * cb] = fmaf(q[h], 0.0625f, o[h]);
                 }
                 tc_fence_before();
-                mbar_arrive(&S.o_empty);
+                if (!dry) mbar_arrive(&S.o_empty);
             }
+            if (dry) {
+                if (pre) pdl_wait();  // the previous step's merge has read the partials
+                dry = false;
+                continue;
+            }
+            cur.next();
+            ++j;
         }
     }
 

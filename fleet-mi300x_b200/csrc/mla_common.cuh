@@ -34,17 +34,18 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Workspace layout (bytes, each region 256-byte aligned).
 //   tiles_cum  int32 [batch + 1]          prefix sum of plan tiles per request (plan_unit_rows)
 //   plan       PlanHeader, PlanEntry [num_ctas]   the split plan per CTA, ready to use (K1 writes it)
-//   qa         bf16  [batch][16][576]     absorbed query q_c (512) | roped q_pe (64), per head
+//   qa         bf16  [batch][16][576]     absorbed query q_c (512) | roped q_pe (64), per head; with
+//              MLA_FLAG_KV8, of the same size, its e4m3 pairs as the split-KV kernel's operand (mla_kv8.cuh)
 //   part_ml    f32   [slots][16][2]       split partial: running max (log2 domain), sum of exps
 //   part_acc   f32   [slots][16][512]     split partial: unnormalised sum_t p_t * c_t
 //   qkv        bf16  [batch][3648]        q | kv_a, when the step projects x_n itself (K0)
-//   qa_lo      bf16  [batch][16][512]     q_c - bf16(q_c), with MLA_FLAG_QC_HILO or MLA_FLAG_KV8
-//   qa_max     f32   [batch][kQMax]       MLA_FLAG_KV8: largest finite |q_c| per 32 columns of a head, then
-//                                         the largest |q_pe| of all heads
+//   qa_lo      bf16  [batch][16][512]     q_c - bf16(q_c), with MLA_FLAG_QC_HILO
+//   q_scale    f32   [batch][32]          MLA_FLAG_KV8: what the pairs are multiplied by: [h] q_c of head h,
+//                                         [16] q_pe of all heads
 // slots = num_ctas + batch: CTA c writes the partial of request b at slot c + b.
 // ---------------------------------------------------------------------------
 struct WsLayout {
-    uint64_t tiles_cum, plan, qa, part_ml, part_acc, qkv, qa_lo, qa_max, total;
+    uint64_t tiles_cum, plan, qa, part_ml, part_acc, qkv, qa_lo, q_scale, total;
     int32_t slots;
 };
 
@@ -65,11 +66,10 @@ __host__ __device__ inline uint64_t align256(uint64_t x) { return (x + 255) & ~u
 
 // with_qkv: the step projects x_n itself (MlaDecodeParams.x_n set), and q | kv_a
 // of every request live in the workspace as [batch][3648] bf16.
-// with_qlo (stores_q_lo): the low half of q_c lives in qa_lo.
-constexpr int kQMaxC = kHeads * (kLora / 32);  // 256
-constexpr int kQMax = kQMaxC + 4;
+// with_qlo: MLA_FLAG_QC_HILO, the low half of q_c lives in qa_lo.
+constexpr int kQScale = 32;  // floats per request in q_scale
 __host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with_qkv = false, bool with_qlo = false,
-                                              bool with_qmax = false) {
+                                              bool kv8 = false) {
     WsLayout w;
     w.slots = num_ctas + batch;
     uint64_t off = 0;
@@ -80,19 +80,14 @@ __host__ __device__ inline WsLayout ws_layout(int batch, int num_ctas, bool with
     w.part_acc = off;  off = align256(off + uint64_t(w.slots) * kHeads * kLora * 4);
     w.qkv = off;       off = align256(off + (with_qkv ? uint64_t(batch) * kQkvRows * 2 : 0));
     w.qa_lo = off;     off = align256(off + (with_qlo ? uint64_t(batch) * kQRows * kLora * 2 : 0));
-    w.qa_max = off;    off = align256(off + (with_qmax ? uint64_t(batch) * kQMax * 4 : 0));
+    w.q_scale = off;   off = align256(off + (kv8 ? uint64_t(batch) * kQScale * 4 : 0));
     w.total = off;
     return w;
 }
 
-// Whether K1 keeps the low half of q_c: the hi/lo form of the default kernel asks for it, and
-// the 8-bit kernel makes its e4m3 pair of q_c from both halves (a pair of the bf16 q_c alone
-// would carry the bf16 rounding, 4x the pair's own).
-__host__ __device__ inline bool stores_q_lo(const MlaDecodeParams& p) {
-    return (p.flags & (MLA_FLAG_QC_HILO | MLA_FLAG_KV8)) != 0;
-}
 __host__ __device__ inline WsLayout ws_layout(const MlaDecodeParams& p) {
-    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, stores_q_lo(p), (p.flags & MLA_FLAG_KV8) != 0);
+    return ws_layout(p.batch, p.num_ctas, p.x_n != nullptr, (p.flags & MLA_FLAG_QC_HILO) != 0,
+                     (p.flags & MLA_FLAG_KV8) != 0);
 }
 
 

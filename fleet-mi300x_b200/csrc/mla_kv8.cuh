@@ -18,6 +18,19 @@ constexpr int kBlocks8 = kPage / kBlock8;            // 4 blocks per page
 constexpr int kPage8 = MLA_PAGE8_BYTES;              // 36,864
 constexpr int kPage8Rope = kPage * kLora;            // offset of the rotary part in a page
 
+// The query of a request as the split-KV kernel's B operand: e4m3 rows n = head (hi) and 16 + head (lo),
+// value = (hi + lo / 16) * q_scale, laid out as it lies in shared memory: [4 column blocks][32 rows]
+// [128 B] with the 128-byte swizzle, then the rotary part [32 rows][64 B] with the 64-byte swizzle.
+constexpr int kQ8N = 2 * kHeads;
+constexpr int kQ8C = kQ8N * kLora, kQ8R = kQ8N * kRope;  // 16,384 and 2,048 bytes
+static_assert(kQ8C + kQ8R == kQRows * kRow * 2, "the image takes the bf16 query's place in the workspace");
+__device__ __forceinline__ int q8_offset(int n, int col) {  // latent column
+    return (col >> 7) * (kQ8N * 128) + n * 128 + ((((col & 127) >> 4) ^ (n & 7)) << 4) + (col & 15);
+}
+__device__ __forceinline__ int q8_offset_rope(int n, int col) {
+    return kQ8C + n * kRope + (((col >> 4) ^ ((n >> 1) & 3)) << 4) + (col & 15);
+}
+
 // The smallest e >= MLA_SCALE_MIN_EXP with amax <= 448 * 2^e = 1.75 * 2^(8 + e), amax finite.
 __device__ __forceinline__ int scale_exponent(float amax) {
     const uint32_t u = __float_as_uint(amax);
@@ -46,6 +59,16 @@ __device__ __forceinline__ float2 from_e4m3x2(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return e4m3x2(a, b) | (e4m3x2(c, d) << 16);
+}
+
+// Two values, |values| <= 448 or NaN, as a pair of e4m3 values each: x = hi + lo / 16 to about 2^-9 of
+// x (its own rounding to f16 on the way is 2^-12). hi and lo hold both values, the first in the low byte.
+__device__ __forceinline__ void e4m3_pairs(float x0, float x1, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x0, x1);
+    hi = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E4M3);
+    const __half2 back(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi, __NV_E4M3));
+    const __half2 r = __hmul2(__hsub2(h, back), __float2half2_rn(16.f));  // exact
+    lo = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(r), __NV_SATFINITE, __NV_E4M3);
 }
 
 // Four stored values, held anew under a scale larger by 1 / f (f a power of two <= 1).

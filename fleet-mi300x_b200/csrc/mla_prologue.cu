@@ -11,7 +11,8 @@
 //    [128 x 128] against a 32 KB slice of W_UK[h] staged by one TMA box; q_nope
 //    and W_UK are bf16 already, so the products are exact; q_c is stored bf16 as
 //    an operand of the attention kernel's score contraction (with
-//    MLA_FLAG_QC_HILO or on an 8-bit cache also its remainder, as a second bf16 array);
+//    MLA_FLAG_QC_HILO also its remainder, as a second bf16 operand); on an 8-bit cache
+//    as e4m3 pairs, in the layout of that kernel's operand;
 //  * the split plan: prefix sum of tiles per request (plan_unit_rows: 32-row half
 //    pages for the default split-KV kernel, 64-row pages for the others), consumed by K2/K3.
 //
@@ -162,7 +163,9 @@ __device__ void request_rows_pre(const MlaDecodeParams& p, int b, int lane, RowP
 
 // One warp, after the wait: q_pe RoPE of request b, then (unless the call stores no
 // row) kv_post + the cache append at local row seq_lens[b].
-__device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b, int lane, const RowPre& r) {
+template <bool kKv8>
+__device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, float* q_scale, int b, int lane,
+                             const RowPre& r) {
     if (!r.ok) return;
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (int64_t)b * p.q_stride;
     __nv_bfloat162 xq[kHeads];
@@ -178,20 +181,39 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
 
     // q_pe of all 16 heads: lane j rotates pair j
     __nv_bfloat16* qrow = qa + (int64_t)b * kQRows * kRow;
-    float qmax = 0.f;
+    if constexpr (kKv8) {  // as e4m3 pairs, under one scale for the request's 16 heads
+        __nv_bfloat162 y[kHeads];  // lo, hi: rotary columns lane and 32 + lane
+        float m = 0.f;
 #pragma unroll
-    for (int h = 0; h < kHeads; ++h) {
-        float lo, hi;
-        rope_pair_r(__low2float(xq[h]), __high2float(xq[h]), r.c0, r.s0, r.c1, r.s1, lo, hi);
-        qrow[h * kRow + kLora + lane] = __float2bfloat16_rn(lo);
-        qrow[h * kRow + kLora + 32 + lane] = __float2bfloat16_rn(hi);
-        qmax = fmaxf(qmax, fmaxf(finite_abs(bf16_round(lo)), finite_abs(bf16_round(hi))));
-    }
-    if (p.flags & MLA_FLAG_KV8) {  // the largest |q_pe|, for its e4m3 scale
+        for (int h = 0; h < kHeads; ++h) {
+            float lo, hi;
+            rope_pair_r(__low2float(xq[h]), __high2float(xq[h]), r.c0, r.s0, r.c1, r.s1, lo, hi);
+            y[h] = __floats2bfloat162_rn(lo, hi);
+            m = fmaxf(m, fmaxf(finite_abs(__low2float(y[h])), finite_abs(__high2float(y[h]))));
+        }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) qmax = fmaxf(qmax, __shfl_xor_sync(0xffffffffu, qmax, o));
-        if (lane == 0)
-            reinterpret_cast<float*>(reinterpret_cast<char*>(p.workspace) + ws_layout(p).qa_max)[(int64_t)b * kQMax + kQMaxC] = qmax;
+        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const int e = scale_exponent(m);
+        const float f = pow2i(-e);
+        uint8_t* img = reinterpret_cast<uint8_t*>(qrow);
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            uint32_t a, b;
+            e4m3_pairs(nan_if_inf(__low2float(y[h])) * f, nan_if_inf(__high2float(y[h])) * f, a, b);
+            img[q8_offset_rope(h, lane)] = (uint8_t)a;
+            img[q8_offset_rope(h, 32 + lane)] = (uint8_t)(a >> 8);
+            img[q8_offset_rope(kHeads + h, lane)] = (uint8_t)b;
+            img[q8_offset_rope(kHeads + h, 32 + lane)] = (uint8_t)(b >> 8);
+        }
+        if (lane == 0) q_scale[(int64_t)b * kQScale + kHeads] = pow2i(e);
+    } else {
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+            float lo, hi;
+            rope_pair_r(__low2float(xq[h]), __high2float(xq[h]), r.c0, r.s0, r.c1, r.s1, lo, hi);
+            qrow[h * kRow + kLora + lane] = __float2bfloat16_rn(lo);
+            qrow[h * kRow + kLora + 32 + lane] = __float2bfloat16_rn(hi);
+        }
     }
     if (!r.append) return;
 
@@ -202,7 +224,7 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
         if (lane == 0) record_error(err_sink(p), MLA_DEV_BAD_PAGE);
         return;
     }
-    if (p.flags & MLA_FLAG_KV8) {  // the same bf16 row, then rounded to e4m3 under its block's scales
+    if constexpr (kKv8) {  // the same bf16 row, then rounded to e4m3 under its block's scales
         RowShare x;
 #pragma unroll
         for (int k = 0; k < 8; ++k) x.c[k] = __nv_bfloat162(outc[2 * k], outc[2 * k + 1]);
@@ -217,12 +239,14 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, int b,
                   outc, lo, hi, lane);
 }
 
+template <bool kKv8>
 __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams p,
                                                             const __grid_constant__ CUtensorMap tmap_wuk) {
     MLA_TL_SCOPE(0);
     const WsLayout ws = ws_layout(p);
     char* wsb = reinterpret_cast<char*>(p.workspace);
     __nv_bfloat16* qa = reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa);
+    float* q_scale = reinterpret_cast<float*>(wsb + ws.q_scale);  // kKv8 only
     const K1Grid g(p.batch);
     const int cta = blockIdx.x;
     extern __shared__ uint8_t smem_raw[];
@@ -247,7 +271,7 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
         pdl_wait();  // q and kv_a come from the previous kernel
         MLA_TL_WAITED(0);
         pdl_trigger();
-        if (c_in < nreq) request_rows(p, qa, b0 + c_in, lane, pre);
+        if (c_in < nreq) request_rows<kKv8>(p, qa, q_scale, b0 + c_in, lane, pre);
         MLA_TL_MARK(0, 5);
         return;  // joins no barrier
     }
@@ -294,6 +318,28 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
         }
     }
     named_bar_sync(1, kK1MmaWarps * 32);  // q_nope staged, barrier initialised
+    // kKv8: a bound of |q_c[b][h][:]|, from which all four CTAs of a head know the same e4m3 scale
+    // without meeting: |q_nope . W_UK[:, l]| <= |q_nope|_2 uk_norm[h] (Cauchy-Schwarz). It lies about
+    // 2 bits above the largest value of a random query; e4m3 pairs have the range for it. Two threads
+    // per request, half a row each, while W_UK is on its way.
+    __shared__ float bound[kReqBlock];
+    if constexpr (kKv8) {
+        const int r = threadIdx.x >> 1, u0 = 8 * (threadIdx.x & 1);
+        float ss = 0.f;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const uint4 v = *reinterpret_cast<const uint4*>(q_s + r * 256 + (((u0 + u) ^ (r & 7)) << 4));
+            const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                ss = fmaf(__low2float(x[i]), __low2float(x[i]), ss);
+                ss = fmaf(__high2float(x[i]), __high2float(x[i]), ss);
+            }
+        }
+        ss += __shfl_xor_sync(0xffffffffu, ss, 1);
+        if (u0 == 0) bound[r] = sqrtf(ss) * p.uk_norm[h] * 1.001f;  // above the roundings of this product and of q_c
+        named_bar_sync(1, kK1MmaWarps * 32);
+    }
     {
         int dummy = 0;
         if (!mbar_wait(bar, 0, &dummy, err_sink(p))) return;
@@ -331,32 +377,54 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
             }
         }
     }
-    // stores_q_lo: the remainder q_c - bf16(q_c), rounded to bf16, into qa_lo
-    __nv_bfloat16* qa_lo = stores_q_lo(p) ? reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa_lo) : nullptr;
+    if constexpr (kKv8) {
+        // Pairs of q_c under the bound's scale, into the operand image; a query that is not finite
+        // has no bound, and its head becomes NaN. Lane t4 collects the 8 columns of latent tile t4 from the
+        // 4 lanes of its row (hi and lo together), so that it stores 8 bytes at a time.
+        uint8_t* img0 = reinterpret_cast<uint8_t*>(qa) + (int64_t)b0 * kQRows * kRow * 2;
+        const int col = kK1LatQ * j + 32 * warp + 8 * t4;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+            if (mt >= n_mt) break;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = 16 * mt + 8 * half + gq;
+                const float m = bound[r];  // rows past the batch are zero
+                const int e = scale_exponent(m);
+                const float f = m <= 3e38f ? pow2i(-e) : __int_as_float(0x7FC00000);
+                uint32_t x[4];  // of tile n: two hi bytes, two lo bytes
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    uint32_t hi, lo;
+                    e4m3_pairs(acc[mt][n][2 * half] * f, acc[mt][n][2 * half + 1] * f, hi, lo);
+                    x[n] = hi | (lo << 16);
+                }
+                // 4 x 4 transposition over the lanes: got[k] = tile t4's bytes from lane k of the row
+                auto pick = [&](int n) { return n & 2 ? (n & 1 ? x[3] : x[2]) : (n & 1 ? x[1] : x[0]); };
+                const uint32_t y0 = pick(t4), y1 = __shfl_xor_sync(0xffffffffu, pick(t4 ^ 1), 1);
+                const uint32_t y2 = __shfl_xor_sync(0xffffffffu, pick(t4 ^ 2), 2);
+                const uint32_t y3 = __shfl_xor_sync(0xffffffffu, pick(t4 ^ 3), 3);  // y_k is from lane t4 ^ k
+                const uint32_t p0 = t4 & 1 ? y1 : y0, p1 = t4 & 1 ? y0 : y1, p2 = t4 & 1 ? y3 : y2, p3 = t4 & 1 ? y2 : y3;
+                const uint32_t got[4] = {t4 & 2 ? p2 : p0, t4 & 2 ? p3 : p1, t4 & 2 ? p0 : p2, t4 & 2 ? p1 : p3};
+                if (r < nreq) {
+                    uint8_t* img = img0 + (int64_t)r * kQRows * kRow * 2;
+                    *reinterpret_cast<uint2*>(img + q8_offset(h, col)) =
+                        make_uint2(__byte_perm(got[0], got[1], 0x5410), __byte_perm(got[2], got[3], 0x5410));
+                    *reinterpret_cast<uint2*>(img + q8_offset(kHeads + h, col)) =
+                        make_uint2(__byte_perm(got[0], got[1], 0x7632), __byte_perm(got[2], got[3], 0x7632));
+                    if (j == 0 && warp == 0 && t4 == 0) q_scale[(int64_t)(b0 + r) * kQScale + h] = pow2i(e);
+                }
+            }
+        }
+        MLA_TL_MARK(0, 4);
+        return;
+    }
+    // MLA_FLAG_QC_HILO: the remainder q_c - bf16(q_c), rounded to bf16, into qa_lo
+    __nv_bfloat16* qa_lo = (p.flags & MLA_FLAG_QC_HILO) ? reinterpret_cast<__nv_bfloat16*>(wsb + ws.qa_lo) : nullptr;
     auto lo2 = [](float x, float y) { return pack_bf16(x - bf16_round(x), y - bf16_round(y)); };
-    // MLA_FLAG_KV8: the largest |q_c| of this warp's 32 columns, per request (the split-KV kernel
-    // then knows its e4m3 scale without a pass over q_c)
-    float* qa_max = (p.flags & MLA_FLAG_KV8) ? reinterpret_cast<float*>(wsb + ws.qa_max) + h * (kLora / 32) + 4 * j + warp
-                                             : nullptr;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
         if (mt >= n_mt) break;
-        if (qa_max) {
-            float m0 = 0.f, m1 = 0.f;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                m0 = fmaxf(m0, fmaxf(finite_abs(acc[mt][n][0]), finite_abs(acc[mt][n][1])));
-                m1 = fmaxf(m1, fmaxf(finite_abs(acc[mt][n][2]), finite_abs(acc[mt][n][3])));
-            }
-#pragma unroll
-            for (int o = 1; o < 4; o <<= 1) {
-                m0 = fmaxf(m0, __shfl_xor_sync(0xffffffffu, m0, o));
-                m1 = fmaxf(m1, __shfl_xor_sync(0xffffffffu, m1, o));
-            }
-            const int r0 = 16 * mt + gq, r1 = r0 + 8;
-            if (t4 == 0 && r0 < nreq) qa_max[(int64_t)(b0 + r0) * kQMax] = m0;
-            if (t4 == 0 && r1 < nreq) qa_max[(int64_t)(b0 + r1) * kQMax] = m1;
-        }
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const int l = kK1LatQ * j + 32 * warp + 8 * n + 2 * t4;
@@ -380,13 +448,43 @@ __global__ void __launch_bounds__(kK1Threads) k1_prologue(const MlaDecodeParams 
     MLA_TL_MARK(0, 4);
 }
 
+// |W_UK[h][:, l]|_2, the largest over the latent columns l, per head: one CTA per head, a thread per two columns.
+__global__ void __launch_bounds__(kLora / 2) k_uk_norms(const __nv_bfloat16* __restrict__ kv_b, float* __restrict__ norms) {
+    __shared__ float red[kLora / 64];
+    const __nv_bfloat162* w = reinterpret_cast<const __nv_bfloat162*>(kv_b + (int64_t)blockIdx.x * kKvbHead * kLora) + threadIdx.x;
+    float a = 0.f, b = 0.f;
+#pragma unroll 8
+    for (int d = 0; d < kNope; ++d) {
+        const __nv_bfloat162 x = w[d * (kLora / 2)];
+        a = fmaf(__low2float(x), __low2float(x), a);
+        b = fmaf(__high2float(x), __high2float(x), b);
+    }
+    a = a <= b ? b : a;  // a NaN in b stays out, one in a stays in: either way q_c has its own
+#pragma unroll
+    for (int o = 16; o; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < kLora / 64; ++i) a = fmaxf(a, red[i]);
+        norms[blockIdx.x] = sqrtf(a);
+    }
+}
+
+cudaError_t launch_uk_norms(const void* kv_b, float* norms, cudaStream_t stream) {
+    k_uk_norms<<<kHeads, kLora / 2, 0, stream>>>(static_cast<const __nv_bfloat16*>(kv_b), norms);
+    return cudaGetLastError();
+}
+
 cudaError_t k1_configure() {
-    return cudaFuncSetAttribute(k1_prologue, cudaFuncAttributeMaxDynamicSharedMemorySize, kK1SmemBytes);
+    const cudaError_t e = cudaFuncSetAttribute(k1_prologue<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kK1SmemBytes);
+    return e != cudaSuccess ? e
+                            : cudaFuncSetAttribute(k1_prologue<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kK1SmemBytes);
 }
 
 cudaError_t launch_prologue(const MlaDecodeParams& p, const CUtensorMap& tmap_wuk, cudaStream_t stream) {
     const K1Grid g(p.batch);
-    return launch_pdl(k1_prologue, dim3(g.total), dim3(kK1Threads), kK1SmemBytes, stream, p, tmap_wuk);
+    return launch_pdl((p.flags & MLA_FLAG_KV8) ? k1_prologue<true> : k1_prologue<false>, dim3(g.total), dim3(kK1Threads),
+                      kK1SmemBytes, stream, p, tmap_wuk);
 }
 
 }  // namespace mla

@@ -48,7 +48,7 @@ EXPORTED = (
     "mla_rows_init", "mla_rows_to_pages", "mla_o_proj", "mla_exchange_bytes", "mla_exchange_alloc",
     "mla_exchange_free", "mla_exchange_open", "mla_exchange_close", "mla_exchange_combine",
     "mla_pool_init", "mla_pool_scratch_size", "mla_pool_fork", "mla_pool_release", "mla_pool_reserve", "mla_pool_compact",
-    "mla_copy_pages",
+    "mla_copy_pages", "mla_uk_norms",
 )
 
 
@@ -95,7 +95,8 @@ class MlaDecodeParams(ctypes.Structure):
         ("exchange", ctypes.c_void_p * MAX_RANKS), ("rank", ctypes.c_int32), ("world", ctypes.c_int32),
         ("exchange_batch", ctypes.c_int32), ("exchange_timeout_us", ctypes.c_int32),
         ("error_host", ctypes.c_void_p),
-        ("kv_scales", ctypes.c_void_p), ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
+        ("kv_scales", ctypes.c_void_p), ("uk_norm", ctypes.c_void_p),
+        ("window", ctypes.c_int32), ("sinks", ctypes.c_int32),
     ]
 
 
@@ -179,7 +180,7 @@ def load_library(path: Path | str | None = None) -> ctypes.CDLL:
         for fn, args in (("mla_pool_scratch_size", [G, ctypes.POINTER(ctypes.c_uint64)]),
                          ("mla_pool_fork", [G, V, V, I, V]), ("mla_pool_release", [G, V, I, V]),
                          ("mla_pool_reserve", [G, V, I, I, V]), ("mla_pool_compact", [G, V]),
-                         ("mla_copy_pages", [G, G, V, V, I, V])):
+                         ("mla_copy_pages", [G, G, V, V, I, V]), ("mla_uk_norms", [V, V, V])):
             getattr(lib, fn).restype = ctypes.c_int
             getattr(lib, fn).argtypes = args
         lib.mla_exchange_bytes.restype = ctypes.c_int

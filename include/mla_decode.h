@@ -110,7 +110,7 @@ typedef enum {
  * or MLA_FLAG_TCGEN05). Each costs tensor-core issue in K2, not HBM bytes. */
 #define MLA_FLAG_QC_HILO 0x20  /* the absorbed query q_c = q_nope W_UK as a bf16 hi/lo pair: K1 writes both halves,
                                   K2 runs the score MMAs of the 512 latent columns on both (about 16 mantissa bits
-                                  of the fp32 q_c instead of 8); the workspace grows by batch x 16 KB (with MLA_FLAG_KV8 too) */
+                                  of the fp32 q_c instead of 8); the workspace grows by batch x 16 KB */
 #define MLA_FLAG_P_HILO 0x40   /* the probabilities of P c_kv as a bf16 hi/lo pair (two MMAs per step) and the row
                                   sums over the unrounded fp32 values, instead of bf16-rounded probabilities */
 
@@ -226,6 +226,8 @@ typedef struct MlaDecodeParams {
     /* ABI v7. */
     void* kv_scales;  /* MLA_FLAG_KV8: int8 [n_pages][4][2], the exponents of each 16-row block of a page
                          (latent part, rotary part), 8-byte aligned; else NULL */
+    const float* uk_norm; /* MLA_FLAG_KV8: f32 [16], per head the largest 2-norm of a column of W_UK
+                         (mla_uk_norms; a property of kv_b, made once with the weights); else NULL */
     int32_t window;   /* sliding window: the query sees the last `window` rows, its own among them; 0 = all.
                          Only the pages that hold a visible row are read. Default and MLA_FLAG_KV8 kernels;
                          not with a sequence-sharded step (MLA_FLAG_NO_NEW_ROW, shard_out, world). */
@@ -348,6 +350,10 @@ typedef struct MlaRowsToPages {
 void mla_rows_init(MlaRowsToPages* r);
 
 int mla_rows_to_pages(const MlaRowsToPages* r, void* stream);
+
+/* norms[h] = max_l |W_UK[h][:, l]|_2 of a layer's kv_b (16 floats, device memory): what a step on an
+ * 8-bit cache takes as uk_norm, to know the scale of its absorbed query ahead of it. Run once per layer. */
+int mla_uk_norms(const void* kv_b, float* norms, void* stream);
 
 /* The life of cache pages (ABI v7): fork, release, reserve, compact and copy, for the caches of
  * all layers of a model in one call (the layers share block_table and seq_lens). The reference keeps

@@ -376,7 +376,7 @@ def test_refusals(cuda_device):
             r.attend(st.q, st.kv_a, cache)
     p = st.runner.params(st.q, st.kv_a, cache, torch.empty(1, 2048, dtype=BF, device=dev))
     for field, value, code in (("kv_scales", None, -1), ("kv_scales", cache.scales.data_ptr() + 4, -3),
-                               ("window", -1, -1), ("sinks", 3, -1)):
+                               ("uk_norm", None, -1), ("window", -1, -1), ("sinks", 3, -1)):
         keep = getattr(p, field)
         setattr(p, field, value)
         assert st.runner.lib.mla_decode_step(p, None) == code, field
