@@ -32,12 +32,14 @@
 // a 32-row step with visible ones, are zeroed in the tile (0 times stale NaN bytes
 // would be NaN).
 //
-// Warps (384 threads):
+// Warps (512 threads):
 //   0      TMA producer: lanes 0 and 1 each load one page of the tile and its exponents
 //   1      score MMAs, owns the tensor memory
 //   2      output MMAs
 //   3      loads the query of the next segment: K1 left it as the operand's image
-//   4-11   softmax: one token and eight heads per thread; partials of a finished segment
+//   4-11   softmax: one token and eight heads per thread
+//   12-15  partials of a finished segment, while the next one runs (its output has the other half of
+//          the tensor memory; written by the softmax warps, a boundary cost about 2.3 us)
 // The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
 // descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
 // clocks of moving them there, elected it takes the 40 that its operands' shared-memory
@@ -53,7 +55,7 @@ namespace mla {
 
 namespace kv8 {
 
-constexpr int kThreads = 384;
+constexpr int kThreads = 512;
 constexpr int kSmWarps = 8;                     // softmax warps: 4 token quarters x 2 halves of the heads
 constexpr int kSmThreads = kSmWarps * 32;
 constexpr int kHh = kHeads / 2;                 // heads of a softmax thread
@@ -78,11 +80,13 @@ struct Smem {
     uint64_t full[kStages], empty[kStages][2];
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_full[2], pv_done[2];
-    uint64_t o_empty, teardown[2];
+    uint64_t o_full[2], o_empty[2];  // a segment's output complete / written out
+    uint64_t ml_full[2];             // its references and row sums
+    uint64_t teardown[2];
     uint64_t exps[kStages][2];  // a page's 4 x 2 exponents
     alignas(16) float q_scale[2][kQScale];  // [buffer]: per head, then the rotary part's
     alignas(16) float red[2][4][16];
-    float lred[4][16];
+    float m_fin[2][16], lred[2][4][16];  // [segment & 1]
     uint32_t tmem_base;
     int abort;
 };
@@ -90,8 +94,8 @@ constexpr int kSmemBytes = kOffMisc + (int)sizeof(Smem) + 1024;  // + alignment 
 static_assert(kSmemBytes <= 232448, "K2 (8-bit) shared memory exceeds 227 KB");
 static_assert(kOffP % 1024 == 0 && kOffQ % 1024 == 0 && kQ % 1024 == 0, "operands must stay 1024-byte aligned");
 
-// Tensor memory columns: two score buffers (latent 32 | rotary 32), four output blocks.
-constexpr int kTmemS = 0, kTmemO = 128, kTmemCols = 256;
+// Tensor memory columns: two score buffers (latent 32 | rotary 32), two outputs of four blocks of 32.
+constexpr int kTmemS = 0, kTmemO = 128, kTmemOSize = 4 * kN, kTmemCols = 512;
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 A/B and fp32 D (the fields of
 // idesc_bf16_f32; format 0 = e4m3).
@@ -271,11 +275,13 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             mbar_init(&S.q_full[i], 1);
             mbar_init(&S.q_empty[i], 1 + kSmWarps);
             mbar_init(&S.s_full[i], 1);
-            mbar_init(&S.p_full[i], kSmThreads);
+            mbar_init(&S.p_full[i], kSmWarps);
             mbar_init(&S.pv_done[i], 1);
             mbar_init(&S.teardown[i], 1);
+            mbar_init(&S.o_full[i], 1);
+            mbar_init(&S.o_empty[i], 4);
+            mbar_init(&S.ml_full[i], kSmWarps);
         }
-        mbar_init(&S.o_empty, kSmThreads);
         S.abort = 0;
         fence_mbar_init();
     } else if (warp == 3 && lane == 0) {
@@ -438,11 +444,13 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), cur.pages(), ks) << ks;
             if (!wait(&S.p_full[sb], (j >> 1) & 1)) break;
-            if (first && cur.seg > 0 && !wait(&S.o_empty, (cur.seg - 1) & 1)) break;
+            const uint32_t ob = cur.seg & 1;
+            if (first && cur.seg >= 2 && !wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1)) break;
             if (!wait(&S.full[st], (j / kStages) & 1)) break;
             tc_fence_after();
             __syncwarp();
             const uint64_t a = dc + ((st * kStageC) >> 4), b = dp + ((sb * kP) >> 4);
+            const bool last = cur.last();
             if (elect_one()) {
                 uint32_t acc = first ? 0u : 1u;
 #pragma unroll
@@ -450,13 +458,14 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     if ((on >> ks) & 1) {
 #pragma unroll
                         for (int cb = 0; cb < 4; ++cb)
-                            mma_f8(tmem + kTmemO + kN * cb, a + ((ks * 4 * kGroup + cb * 1024) >> 4),
+                            mma_f8(tmem + kTmemO + ob * kTmemOSize + kN * cb, a + ((ks * 4 * kGroup + cb * 1024) >> 4),
                                    b + ((ks * 32 * kN) >> 4), kIdescPV, acc);
                         acc = 1u;
                     }
                     if (ks & 1) tc_commit(&S.empty[st][ks >> 1]);
                 }
                 tc_commit(&S.pv_done[sb]);
+                if (last) tc_commit(&S.o_full[ob]);
             }
             __syncwarp();
         }
@@ -484,19 +493,53 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 if (fills) mbar_drain(&S.q_full[qb], (fills - 1) & 1, err);
             }
         }
-    } else if (warp >= 4) {
-        // ------------------------------------------------------------ softmax, partials
-        const int sp = warp & 3, tok = 32 * sp + lane, half = tok >> 6, slot = tok & (kPage - 1);
-        const int h0 = warp < 8 ? 0 : kHh;  // this thread's heads: h0 .. h0 + 7
+    } else if (warp >= 12) {
+        // ------------------------------------------------------------ partials
+        // Thread: latent column 32 sp + lane of each 128-column block, all 16 heads.
+        const int sp = warp & 3;
         float* part_ml = reinterpret_cast<float*>(wsb + ws.part_ml);
         float* part_acc = reinterpret_cast<float*>(wsb + ws.part_acc);
+        if (pre) pdl_wait();  // the previous step's merge has read the partials
+        for (; cur.valid(); cur.next_request()) {
+            const uint32_t ob = cur.seg & 1, ph = (cur.seg >> 1) & 1;
+            const int64_t part = (int64_t)vc + cur.b;
+            wait(&S.ml_full[ob], ph);
+            if (sp == 0 && lane < kHeads) {
+                const float l = (S.lred[ob][0][lane] + S.lred[ob][1][lane]) + (S.lred[ob][2][lane] + S.lred[ob][3][lane]);
+                *reinterpret_cast<float2*>(part_ml + (part * kHeads + lane) * 2) = make_float2(S.m_fin[ob][lane], l);
+            }
+            __syncwarp();
+            wait(&S.o_full[ob], ph);
+            tc_fence_after();
+            __syncwarp();
+            float* acc = part_acc + part * kHeads * kLora + 32 * sp + lane;
+#pragma unroll 2
+            for (int k = 0; k < 8; ++k) {  // four blocks, two halves of the heads
+                float o[kHh], q[kHh];
+                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + ob * kTmemOSize + kN * (k >> 1) + kHh * (k & 1));
+                tmem_ld8(ta, o);
+                tmem_ld8(ta + kHeads, q);
+                tmem_wait_ld();
+                loaded(o); loaded(q);
+#pragma unroll
+                for (int h = 0; h < kHh; ++h)
+                    acc[(kHh * (k & 1) + h) * kLora + 128 * (k >> 1)] = fmaf(q[h], 0.0625f, o[h]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.o_empty[ob]);
+        }
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ softmax
+        const int sp = warp & 3, tok = 32 * sp + lane, half = tok >> 6, slot = tok & (kPage - 1);
+        const int h0 = warp < 8 ? 0 : kHh;  // this thread's heads: h0 .. h0 + 7
         float m[kHh], l[kHh];  // reference (log2 domain), this thread's part of the row sum
         float qs[kHh], qsr = 0.f;  // what this thread's heads' scores are multiplied by, latent and rotary
         Visible vis;
         uint32_t j = 0;
         // The first pass is a rehearsal without a visible row, while the first tile is on its way: it
         // fetches the code (measured: 3,000 clocks for a first tile from a cold cache, 1,000 for a later
-        // one). It waits for nothing, signals nothing and stores nothing outside the P buffer.
+        // one). It waits for nothing, signals nothing and stores nothing that is not written again.
         for (bool dry = true; dry || cur.valid();) {
             const uint32_t st = j % kStages, sb = j & 1;
             const bool first = cur.first(), last = cur.last();
@@ -572,7 +615,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
 #pragma unroll 2
                     for (int k = 0; k < 8; ++k) {  // four blocks, hi and lo
                         float o[kHh];
-                        const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + 16 * k + h0);
+                        const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + (cur.seg & 1) * kTmemOSize + 16 * k + h0);
                         tmem_ld8(ta, o);
                         tmem_wait_ld();
                         loaded(o);
@@ -615,42 +658,22 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             }
             fence_proxy_async_smem();
             tc_fence_before();
-            if (!dry) mbar_arrive(&S.p_full[sb]);
+            __syncwarp();
+            if (!dry && lane == 0) mbar_arrive(&S.p_full[sb]);
 
-            if (last || dry) {
+            if (last || dry) {  // the segment's references and row sums, for the partial
+                const uint32_t ob = cur.seg & 1;
                 const float ls = reduce8<false>(l, lane);
-                if ((lane & 3) == 0) S.lred[sp][h0 + (lane >> 2)] = ls;
-                named_bar_sync(1, kSmThreads);
-                const int64_t part = (int64_t)vc + cur.b;
-                if (sp == 0 && lane < kHh && !dry) {
-                    float mh = 0.f;
+                if (cur.seg >= 2) wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1);
+                if ((lane & 3) == 0) S.lred[ob][sp][h0 + (lane >> 2)] = ls;
+                if (sp == 0 && lane == 0) {
 #pragma unroll
-                    for (int h = 0; h < kHh; ++h) if (h == lane) mh = m[h];
-                    const int h = h0 + lane;
-                    const float lh = (S.lred[0][h] + S.lred[1][h]) + (S.lred[2][h] + S.lred[3][h]);
-                    *reinterpret_cast<float2*>(part_ml + (part * kHeads + h) * 2) = make_float2(mh, lh);
+                    for (int h = 0; h < kHh; ++h) S.m_fin[ob][h0 + h] = m[h];
                 }
                 __syncwarp();
-                if (!dry) wait(&S.pv_done[sb], (j >> 1) & 1);
-                tc_fence_after();
-                __syncwarp();
-                float* acc = part_acc + (part * kHeads + h0) * kLora + 32 * sp + lane;
-#pragma unroll
-                for (int cb = 0; cb < 4; ++cb) {
-                    float o[kHh], q[kHh];
-                    tmem_ld8(tmem_lane_addr(tmem, sp, kTmemO + kN * cb + h0), o);
-                    tmem_ld8(tmem_lane_addr(tmem, sp, kTmemO + kN * cb + 16 + h0), q);
-                    tmem_wait_ld();
-                    loaded(o); loaded(q);
-#pragma unroll
-                    for (int h = 0; h < kHh; ++h)
-                        if (!dry) acc[h * kLora + 128 * cb] = fmaf(q[h], 0.0625f, o[h]);
-                }
-                tc_fence_before();
-                if (!dry) mbar_arrive(&S.o_empty);
+                if (!dry && lane == 0) mbar_arrive(&S.ml_full[ob]);
             }
             if (dry) {
-                if (pre) pdl_wait();  // the previous step's merge has read the partials
                 dry = false;
                 continue;
             }
