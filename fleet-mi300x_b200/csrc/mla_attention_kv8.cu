@@ -8,11 +8,10 @@
 //
 // Why tensor memory here and m16n8k16 on the bf16 cache: with half the bytes per row
 // the SM has half the time per row (25 clocks at the copy peak), and m16n8k16 would
-// spend 70 % of its issue on it before a single conversion. An f8f6f4 MMA takes a
-// tile of 128 tokens x 32 bytes whatever its N (measured: 60 clocks per issued MMA at
-// N = 16 and N = 32, M = 64 and 128, one issuing thread), so 128 tokens x 16 heads
-// cost 18 + 16 MMAs, which two issuing threads keep under a third of the tile's HBM
-// time (about 3,300 clocks). N is nearly free, so it carries precision: an operand
+// spend 70 % of its issue on it before a single conversion. An f8f6f4 MMA of K = 32 bytes and
+// N = 32 takes 40 clocks at M = 128 and 26 at M = 64 (measured: its shared-memory reads at 128 B
+// per clock), so 128 tokens x 16 heads cost 36 + 16 MMAs, 1,570 of the about 3,300 clocks of
+// their HBM time. N is nearly free, so it carries precision: an operand
 // that is not 8 bits already enters as a pair of e4m3 values side by side on N,
 // x = hi + lo / 16, about as precise as bf16 (8 significant bits):
 //   scores  S^T[t][hi 16 | lo 16]  = C[t][:] . Q[hi | lo]   (latent and rotary apart: their scales differ)
@@ -27,13 +26,13 @@
 // rescale reads and writes O in tensor memory, which happens in the first few tiles
 // of a segment only). Sums, scores and the output are fp32.
 //
-// Tiles of up to two 64-row pages of a request (the plan's units are pages), TMA'd
-// into a ring of two; rows that the query does not see have P' = 0 and, if they share
-// a 32-row step with visible ones, are zeroed in the tile (0 times stale NaN bytes
-// would be NaN).
+// Pages (the plan's units) are TMA'd into a ring of five; a tile is up to two pages of a request. The
+// scores are M = 64 MMAs per page, so that a page needs no neighbour in the ring and its scores start
+// when it lands. Rows that the query does not see have P' = 0 and, if they share a 32-row step with
+// visible ones, are zeroed in the ring (0 times stale NaN bytes would be NaN).
 //
 // Warps (512 threads):
-//   0      TMA producer: lanes 0 and 1 each load one page of the tile and its exponents
+//   0      TMA producer: pages and their exponents
 //   1      score MMAs, owns the tensor memory
 //   2      output MMAs
 //   3      loads the query of the next segment: K1 left it as the operand's image
@@ -42,8 +41,7 @@
 //          the tensor memory; written by the softmax warps, a boundary cost about 2.3 us)
 // The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
 // descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
-// clocks of moving them there, elected it takes the 40 that its operands' shared-memory
-// reads need (5 KB at 128 B per clock).
+// clocks of moving them there.
 // Every wait is bounded: a stall records MLA_DEV_TIMEOUT, the roles fall through
 // their remaining waits, copies and MMAs drain and the tensor memory is freed.
 #include <cuda.h>
@@ -59,34 +57,34 @@ constexpr int kThreads = 512;
 constexpr int kSmWarps = 8;                     // softmax warps: 4 token quarters x 2 halves of the heads
 constexpr int kSmThreads = kSmWarps * 32;
 constexpr int kHh = kHeads / 2;                 // heads of a softmax thread
-constexpr int kStages = 2;
+constexpr int kSlots = 5;                       // ring of pages
+constexpr int kEarly = 2;                       // pages requested before the wait on K1
 constexpr int kTok = 2 * kPage;                 // tokens per tile
 constexpr int kGroup = 8 * kLora;               // 4096: 8 rows of the latent part, [4 column blocks][8][128 B]
-constexpr int kHalfC = kPage * kLora;           // one page's latent bytes in a stage
-constexpr int kHalfR = kPage * kRope;
-constexpr int kStageC = 2 * kHalfC;             // 65,536
-constexpr int kStageR = 2 * kHalfR;             // 8,192
+constexpr int kSlotC = kPage * kLora;           // 32,768
+constexpr int kSlotR = kPage * kRope;           // 4,096
 constexpr int kN = kQ8N;                        // hi | lo
 constexpr int kQ = kQ8C + kQ8R;                 // a request's query image
 constexpr int kP = kTok * kN;                   // [128 tokens][32 B]
 
 constexpr int kOffC = 0;
-constexpr int kOffR = kOffC + kStages * kStageC;
-constexpr int kOffQ = kOffR + kStages * kStageR;
+constexpr int kOffR = kOffC + kSlots * kSlotC;
+constexpr int kOffQ = kOffR + kSlots * kSlotR;
 constexpr int kOffP = kOffQ + 2 * kQ;
 constexpr int kOffMisc = kOffP + 2 * kP;
 
 struct Smem {
-    uint64_t full[kStages], empty[kStages][2];
+    uint64_t full[kSlots], empty[kSlots];
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_full[2], pv_done[2];
     uint64_t o_full[2], o_empty[2];  // a segment's output complete / written out
     uint64_t ml_full[2];             // its references and row sums
     uint64_t teardown[2];
-    uint64_t exps[kStages][2];  // a page's 4 x 2 exponents
+    uint64_t exps[kSlots];  // a page's 4 x 2 exponents
     alignas(16) float q_scale[2][kQScale];  // [buffer]: per head, then the rotary part's
     alignas(16) float red[2][4][16];
     float m_fin[2][16], lred[2][4][16];  // [segment & 1]
+    int32_t pre_cum[65];
     uint32_t tmem_base;
     int abort;
 };
@@ -94,8 +92,10 @@ constexpr int kSmemBytes = kOffMisc + (int)sizeof(Smem) + 1024;  // + alignment 
 static_assert(kSmemBytes <= 232448, "K2 (8-bit) shared memory exceeds 227 KB");
 static_assert(kOffP % 1024 == 0 && kOffQ % 1024 == 0 && kQ % 1024 == 0, "operands must stay 1024-byte aligned");
 
-// Tensor memory columns: two score buffers (latent 32 | rotary 32), two outputs of four blocks of 32.
-constexpr int kTmemS = 0, kTmemO = 128, kTmemOSize = 4 * kN, kTmemCols = 512;
+// Tensor memory columns: two score buffers (per page of the tile: latent 32 | rotary 32), two outputs of four
+// blocks of 32. The scores of a page (M = 64) lie in lanes 0-15 of each warp's 32.
+constexpr int kTmemS = 0, kTmemSPage = 2 * kN, kTmemSSize = 2 * kTmemSPage;
+constexpr int kTmemO = 2 * kTmemSSize, kTmemOSize = 4 * kN, kTmemCols = 512;
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 A/B and fp32 D (the fields of
 // idesc_bf16_f32; format 0 = e4m3).
@@ -103,7 +103,7 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, int a_mn_major, 
     return (1u << 4) | (uint32_t(a_mn_major) << 15) | (uint32_t(b_mn_major) << 16) | (uint32_t(N >> 3) << 17) |
            (uint32_t(M >> 4) << 24);
 }
-constexpr uint32_t kIdescQK = idesc_e4m3(128, kN, 0, 0);
+constexpr uint32_t kIdescQK = idesc_e4m3(64, kN, 0, 0);
 constexpr uint32_t kIdescPV = idesc_e4m3(128, kN, 1, 1);
 
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -175,11 +175,17 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-// 32 lanes x 8 consecutive tensor-memory columns (tmem_ld16, half as wide), and back.
+// 8 consecutive tensor-memory columns of 32 lanes (tmem_ld16, half as wide), and back.
 __device__ __forceinline__ void tmem_ld8(uint32_t taddr, float (&v)[kHh]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                  : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
                  : "r"(taddr));
+}
+// 8 score columns of a warp's 16 rows of either page: threads 0-15 the first page's, 16-31 the second's.
+__device__ __forceinline__ void tmem_ld8_pages(uint32_t taddr, float (&v)[kHh]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8], %9;"
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                 : "r"(taddr), "n"(kTmemSPage));
 }
 // The loaded values, not to be used before the tmem_wait_ld that precedes this call.
 __device__ __forceinline__ void loaded(float (&v)[kHh]) {
@@ -246,7 +252,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
     // the split plan: for up to 64 requests from the step's inputs, before the wait on K1 (the rule
     // K1's planner uses); beyond, all read K1's plan entry after it.
     constexpr int kPrePlan = 64;
-    __shared__ int32_t pre_cum[kPrePlan + 1];
+    int32_t* pre_cum = S.pre_cum;
     const bool pre = p.batch <= kPrePlan;
     if (warp == 0) {
         if (pre) {
@@ -266,10 +272,9 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         tmem_alloc(&S.tmem_base, kTmemCols);
         tmem_relinquish();
     } else if (warp == 2 && lane == 0) {
-        for (int i = 0; i < kStages; ++i) {
-            mbar_init(&S.full[i], 2);
-            mbar_init(&S.empty[i][0], 1);
-            mbar_init(&S.empty[i][1], 1);
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&S.full[i], 1);
+            mbar_init(&S.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&S.q_full[i], 1);
@@ -334,64 +339,49 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer
-        // Lane l (0, 1) loads page l of each tile. The page id is loaded two tiles ahead
-        // and the exponents one tile ahead, so that neither latency is on the path.
-        if (lane < 2) {
+        // A page's number is loaded two pages ahead and its exponents one page ahead, so that
+        // neither latency is on the path. Up to kEarly pages go out before the wait on K1, none that
+        // K1 appends to (and whose exponents it may raise).
+        if (lane == 0) {
+            struct Page { int id; bool appended; };
+            TileCursor la = cur;  // two pages ahead of the one being loaded
             Visible vis;
-            auto page_of = [&](const Walk& w) -> int {
-                if (w.first()) vis = visible(w.b);
-                if (!w.valid() || lane >= w.pages()) return -1;  // no page for this lane
-                int pg = p.block_table[(int64_t)w.b * p.max_blocks + vis.tile(w.index() + lane)];
-                if (pg < 0 || pg >= p.n_pages) { record_error(err, MLA_DEV_BAD_PAGE); pg = 0; }
-                return pg;
+            auto page_of = [&]() -> Page {
+                if (la.first()) vis = visible(la.b);
+                const int k = vis.tile(la.index());
+                int id = p.block_table[(int64_t)la.b * p.max_blocks + k];
+                if (id < 0 || id >= p.n_pages) { record_error(err, MLA_DEV_BAD_PAGE); id = 0; }
+                return Page{id, fresh && k == (vis.rows - 1) / kPage};
             };
-            auto exps_of = [&](int pg) -> uint64_t {
-                return pg < 0 ? 0ull : reinterpret_cast<const uint64_t*>(p.kv_scales)[pg];
-            };
-            uint32_t issued = 0;
-            auto issue = [&](uint32_t j, int pg, uint64_t ex) {
-                const uint32_t st = j % kStages;
-                S.exps[st][lane] = ex;
-                if (pg < 0) {
-                    mbar_arrive(&S.full[st]);
-                } else {
-                    mbar_arrive_expect_tx(&S.full[st], kHalfC + kHalfR);
-                    tma_load_5d(smem + kOffC + st * kStageC + lane * kHalfC, &tmap_c, &S.full[st], 0, 0, 0, 0, pg,
-                                kCacheEvictFirst);
-                    tma_load_3d(smem + kOffR + st * kStageR + lane * kHalfR, &tmap_r, &S.full[st], 0, 0, pg,
-                                kCacheEvictFirst);
-                }
-                ++issued;
-            };
-            int pg0 = page_of(cur);
-            bool early = false;
-            if (pre) {  // the first page before the wait, unless it is the one K1 appends to
-                const bool holds_new = fresh && pg0 >= 0 && vis.tile(cur.index() + lane) == (vis.rows - 1) / kPage;
-                if (!holds_new) {
-                    issue(0, pg0, exps_of(pg0));
-                    early = true;
-                }
-            }
-            Walk la = cur;  // two tiles ahead of the one being loaded
+            auto exps_of = [&](int id) { return reinterpret_cast<const uint64_t*>(p.kv_scales)[id]; };
+            bool waited = !pre;
+            Page p0 = page_of(), p1 = p0, p2 = p0;
             la.next();
-            int pg1 = la.valid() ? page_of(la) : -1;
-            if (pre) { pdl_wait(); MLA_TL_WAITED(1); }
-            uint64_t ex0 = exps_of(pg0);
-            uint32_t j = 0;
-            for (; cur.valid(); cur.next(), ++j) {
+            if (la.valid()) p1 = page_of();
+            uint64_t ex0 = exps_of(p0.id), ex1 = ex0;
+            bool early0 = !waited, early1 = early0;  // loaded before the wait
+            uint32_t i = 0;
+            TileCursor at = cur;
+            for (; at.valid(); at.next(), ++i) {
+                if (!waited && (i >= kEarly || p0.appended)) { pdl_wait(); MLA_TL_WAITED(1); waited = true; }
+                if (p0.appended && early0) ex0 = exps_of(p0.id);
                 la.next();
-                const int pg2 = la.valid() ? page_of(la) : -1;
-                const uint64_t ex1 = exps_of(pg1);
-                if (!(j == 0 && early)) {
-                    if (j >= kStages && !wait(&S.empty[j % kStages][lane], (j / kStages - 1) & 1)) break;
-                    issue(j, pg0, ex0);
-                }
-                pg0 = pg1; pg1 = pg2; ex0 = ex1;
+                if (la.valid()) p2 = page_of();
+                ex1 = exps_of(p1.id);
+                early1 = !waited;
+                const uint32_t sl = i % kSlots;
+                if (i >= kSlots && !wait(&S.empty[sl], (i / kSlots - 1) & 1)) break;
+                S.exps[sl] = ex0;
+                mbar_arrive_expect_tx(&S.full[sl], kSlotC + kSlotR);
+                tma_load_5d(smem + kOffC + sl * kSlotC, &tmap_c, &S.full[sl], 0, 0, 0, 0, p0.id, kCacheEvictFirst);
+                tma_load_3d(smem + kOffR + sl * kSlotR, &tmap_r, &S.full[sl], 0, 0, p0.id, kCacheEvictFirst);
+                p0 = p1; p1 = p2; ex0 = ex1; early0 = early1;
             }
+            if (!waited) pdl_wait();
             // Drain: every issued copy must land before the CTA's shared memory is released.
-            for (uint32_t st = 0; st < kStages; ++st) {
-                const uint32_t fills = issued / kStages + (st < issued % kStages ? 1u : 0u);
-                if (fills) mbar_drain(&S.full[st], (fills - 1) & 1, err);
+            for (uint32_t sl = 0; sl < kSlots; ++sl) {
+                const uint32_t fills = i / kSlots + (sl < i % kSlots ? 1u : 0u);
+                if (fills) mbar_drain(&S.full[sl], (fills - 1) & 1, err);
             }
         }
     } else if (warp == 1) {
@@ -400,30 +390,37 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         const uint64_t dr = desc_of(smem_u32(smem + kOffR), 8 * kRope, kSw64);
         const uint64_t dqc = desc_of(smem_u32(smem + kOffQ), 1024, kSw128);
         const uint64_t dqr = desc_of(smem_u32(smem + kOffQ + kQ8C), 8 * kRope, kSw64);
-        uint32_t j = 0;
-        for (; cur.valid(); cur.next(), ++j) {
-            const uint32_t st = j % kStages, qb = cur.seg & 1, sb = j & 1;
-            if (cur.first() && !wait(&S.q_full[qb], (cur.seg >> 1) & 1)) break;
-            if (!wait(&S.full[st], (j / kStages) & 1)) break;
-            if (j >= 2 && !wait(&S.p_full[sb], ((j - 2) >> 1) & 1)) break;  // the buffer's scores were read
-            tc_fence_after();
-            __syncwarp();
-            const uint64_t a = dc + ((st * kStageC) >> 4), b = dqc + ((qb * kQ) >> 4);
-            const uint64_t ar = dr + ((st * kStageR) >> 4), br = dqr + ((qb * kQ) >> 4);
-            const uint32_t d = tmem + kTmemS + 64 * sb;
+        uint32_t j = 0, i = 0;  // tile, page
+        bool ok = true;
+        for (; ok && cur.valid(); cur.next(), ++j) {
+            const uint32_t qb = cur.seg & 1, sb = j & 1;
+            const int pages = cur.pages();
             const bool last = cur.last();
-            if (elect_one()) {
+            if (cur.first() && !wait(&S.q_full[qb], (cur.seg >> 1) & 1)) break;
+            if (j >= 2 && !wait(&S.p_full[sb], ((j - 2) >> 1) & 1)) break;  // the buffer's scores were read
+            const uint64_t b = dqc + ((qb * kQ) >> 4), br = dqr + ((qb * kQ) >> 4);
+            for (int k = 0; k < pages; ++k, ++i) {
+                const uint32_t sl = i % kSlots;
+                if (!(ok = wait(&S.full[sl], (i / kSlots) & 1))) break;
+                tc_fence_after();
+                __syncwarp();
+                const uint64_t a = dc + ((sl * kSlotC) >> 4), ar = dr + ((sl * kSlotR) >> 4);
+                const uint32_t d = tmem + kTmemS + kTmemSSize * sb + kTmemSPage * k;
+                if (elect_one()) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    mma_f8(d, a + (((i >> 2) * 1024 + (i & 3) * 32) >> 4),
-                           b + (((i >> 2) * (kN * 128) + (i & 3) * 32) >> 4), kIdescQK, i > 0);
+                    for (int x = 0; x < 16; ++x)
+                        mma_f8(d, a + (((x >> 2) * 1024 + (x & 3) * 32) >> 4),
+                               b + (((x >> 2) * (kN * 128) + (x & 3) * 32) >> 4), kIdescQK, x > 0);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    mma_f8(d + kN, ar + ((i * 32) >> 4), br + ((i * 32) >> 4), kIdescQK, i > 0);
-                tc_commit(&S.s_full[sb]);
-                if (last) tc_commit(&S.q_empty[qb]);
+                    for (int x = 0; x < 2; ++x)
+                        mma_f8(d + kN, ar + ((x * 32) >> 4), br + ((x * 32) >> 4), kIdescQK, x > 0);
+                    if (k == pages - 1) {
+                        tc_commit(&S.s_full[sb]);
+                        if (last) tc_commit(&S.q_empty[qb]);
+                    }
+                }
+                __syncwarp();
             }
-            __syncwarp();
         }
         __syncwarp();
         if (elect_one()) {  // all issued MMAs complete before the tensor memory is freed
@@ -435,34 +432,37 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         const uint64_t dc = desc_of(smem_u32(smem + kOffC), kGroup, kSw128);
         const uint64_t dp = desc_of(smem_u32(smem + kOffP), 8 * kN, kSw32);
         Visible vis;
-        uint32_t j = 0;
-        for (; cur.valid(); cur.next(), ++j) {
-            const uint32_t st = j % kStages, sb = j & 1;
-            const bool first = cur.first();
+        uint32_t j = 0, i = 0;
+        for (; cur.valid(); i += cur.pages(), cur.next(), ++j) {
+            const uint32_t sb = j & 1, ob = cur.seg & 1;
+            const bool first = cur.first(), last = cur.last();
+            const int pages = cur.pages();
             if (first) vis = visible(cur.b);
             uint32_t on = 0;  // bit ks: the 32-row step ks holds a visible row
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), cur.pages(), ks) << ks;
+            for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), pages, ks) << ks;
+            const uint32_t sl0 = i % kSlots, sl1 = (i + 1) % kSlots;
             if (!wait(&S.p_full[sb], (j >> 1) & 1)) break;
-            const uint32_t ob = cur.seg & 1;
             if (first && cur.seg >= 2 && !wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1)) break;
-            if (!wait(&S.full[st], (j / kStages) & 1)) break;
+            if (!wait(&S.full[sl0], (i / kSlots) & 1)) break;
+            if (pages > 1 && !wait(&S.full[sl1], ((i + 1) / kSlots) & 1)) break;
             tc_fence_after();
             __syncwarp();
-            const uint64_t a = dc + ((st * kStageC) >> 4), b = dp + ((sb * kP) >> 4);
-            const bool last = cur.last();
+            const uint64_t a0 = dc + ((sl0 * kSlotC) >> 4), a1 = dc + ((sl1 * kSlotC) >> 4), b = dp + ((sb * kP) >> 4);
+            const uint32_t d = tmem + kTmemO + ob * kTmemOSize;
             if (elect_one()) {
                 uint32_t acc = first ? 0u : 1u;
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                     if ((on >> ks) & 1) {
+                        const uint64_t a = (ks < 2 ? a0 : a1) + (((ks & 1) * 4 * kGroup) >> 4);
 #pragma unroll
                         for (int cb = 0; cb < 4; ++cb)
-                            mma_f8(tmem + kTmemO + ob * kTmemOSize + kN * cb, a + ((ks * 4 * kGroup + cb * 1024) >> 4),
-                                   b + ((ks * 32 * kN) >> 4), kIdescPV, acc);
+                            mma_f8(d + kN * cb, a + ((cb * 1024) >> 4), b + ((ks * 32 * kN) >> 4), kIdescPV, acc);
                         acc = 1u;
                     }
-                    if (ks & 1) tc_commit(&S.empty[st][ks >> 1]);
+                    if (ks == 1) tc_commit(&S.empty[sl0]);
+                    if (ks == 3 && pages > 1) tc_commit(&S.empty[sl1]);
                 }
                 tc_commit(&S.pv_done[sb]);
                 if (last) tc_commit(&S.o_full[ob]);
@@ -531,23 +531,27 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         }
     } else if (warp >= 4) {
         // ------------------------------------------------------------ softmax
-        const int sp = warp & 3, tok = 32 * sp + lane, half = tok >> 6, slot = tok & (kPage - 1);
+        // Threads 0-15 of a warp hold rows 16 sp .. of the tile's first page, 16-31 those of the second.
+        const int sp = warp & 3, half = lane >> 4, slot = 16 * sp + (lane & 15), tok = half * kPage + slot;
         const int h0 = warp < 8 ? 0 : kHh;  // this thread's heads: h0 .. h0 + 7
         float m[kHh], l[kHh];  // reference (log2 domain), this thread's part of the row sum
         float qs[kHh], qsr = 0.f;  // what this thread's heads' scores are multiplied by, latent and rotary
         Visible vis;
-        uint32_t j = 0;
+        uint32_t j = 0, i0 = 0;  // tile, its first page
         // The first pass is a rehearsal without a visible row, while the first tile is on its way: it
         // fetches the code (measured: 3,000 clocks for a first tile from a cold cache, 1,000 for a later
         // one). It waits for nothing, signals nothing and stores nothing that is not written again.
         for (bool dry = true; dry || cur.valid();) {
-            const uint32_t st = j % kStages, sb = j & 1;
+            const uint32_t sb = j & 1, sl0 = i0 % kSlots, sl1 = (i0 + 1) % kSlots, sl = half ? sl1 : sl0;
             const bool first = cur.first(), last = cur.last();
             if (first) vis = visible(cur.b);
             const int index = cur.index(), pages = cur.pages();
             const bool sees = !dry && half < pages && vis.row(kPage * vis.tile(index + half) + slot);
-            if (!dry) wait(&S.full[st], (j / kStages) & 1);  // the exponents, and the tile itself where rows are zeroed
-            const char2 ex = sees ? reinterpret_cast<const char2*>(&S.exps[st][half])[slot / kBlock8] : make_char2(0, 0);
+            if (!dry) {  // the exponents, and the pages themselves where rows are zeroed
+                wait(&S.full[sl0], (i0 / kSlots) & 1);
+                if (pages > 1) wait(&S.full[sl1], ((i0 + 1) / kSlots) & 1);
+            }
+            const char2 ex = sees ? reinterpret_cast<const char2*>(&S.exps[sl])[slot / kBlock8] : make_char2(0, 0);
             if (first) {
                 const int qb = cur.seg & 1;
                 if (!dry) wait(&S.q_full[qb], (cur.seg >> 1) & 1);
@@ -566,11 +570,11 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             float s[kHh];
             {
                 float a[kHh], b[kHh], c[kHh];
-                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemS + 64 * sb + h0);
-                tmem_ld8(ta, s);
-                tmem_ld8(ta + 16, a);
-                tmem_ld8(ta + 32, b);
-                tmem_ld8(ta + 48, c);
+                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemS + kTmemSSize * sb + h0);
+                tmem_ld8_pages(ta, s);
+                tmem_ld8_pages(ta + 16, a);
+                tmem_ld8_pages(ta + 32, b);
+                tmem_ld8_pages(ta + 48, c);
                 tmem_wait_ld();
                 loaded(s); loaded(a); loaded(b); loaded(c);
 #pragma unroll
@@ -650,8 +654,8 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 *reinterpret_cast<uint2*>(pt + (sw << 4)) = make_uint2(hi[0], hi[1]);
                 *reinterpret_cast<uint2*>(pt + ((sw ^ 1) << 4)) = make_uint2(lo[0], lo[1]);
             }
-            if (!sees && !dry && step_on(vis, index, pages, sp)) {  // 0 * stale bytes must be 0
-                uint8_t* row = smem + kOffC + st * kStageC + (tok >> 3) * kGroup + (tok & 7) * 128 + (h0 >> 3) * 2048;
+            if (!sees && !dry && step_on(vis, index, pages, 2 * half + (slot >> 5))) {  // 0 * stale bytes must be 0
+                uint8_t* row = smem + kOffC + sl * kSlotC + (slot >> 3) * kGroup + (slot & 7) * 128 + (h0 >> 3) * 2048;
 #pragma unroll 4
                 for (int i = 0; i < kLora / 32; ++i)  // this half's two column blocks
                     *reinterpret_cast<uint4*>(row + (i >> 3) * 1024 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
@@ -677,6 +681,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                 dry = false;
                 continue;
             }
+            i0 += pages;
             cur.next();
             ++j;
         }
