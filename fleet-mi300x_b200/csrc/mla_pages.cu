@@ -82,6 +82,28 @@ __device__ int block_scan(int v, int* warp_tot, int& total) {
     return before + incl - v;
 }
 
+// Whether some request is named twice among ids[0, n) (numbers outside the batch do not count), by a
+// bitmap in shared memory: in the usual case that no owner has to be found through global memory.
+__device__ bool named_twice(const MlaPagePool& p, const int32_t* __restrict__ ids, int n, uint32_t* seen) {
+    for (int i = threadIdx.x; i < (p.batch + 31) / 32; i += kPlanThreads) seen[i] = 0;
+    __syncthreads();
+    bool twice = false;
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) {
+        const int b = ids[i];
+        if (b >= 0 && b < p.batch) twice |= (atomicOr(&seen[b >> 5], 1u << (b & 31)) >> (b & 31)) & 1;
+    }
+    return __syncthreads_or(twice);
+}
+// Then: owner[b] = the last i with ids[i] = b.
+__device__ void last_named(const MlaPagePool& p, const int32_t* __restrict__ ids, int n, int32_t* owner) {
+    for (int i = threadIdx.x; i < n; i += kPlanThreads)
+        if (ids[i] >= 0 && ids[i] < p.batch) owner[ids[i]] = -1;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kPlanThreads)
+        if (ids[i] >= 0 && ids[i] < p.batch) atomicMax(&owner[ids[i]], i);
+    __syncthreads();
+}
+
 // The pages of [from, to) that are free (live = false) or held, in order, the first
 // `want` of them into ids; returns how many were found (the same in every thread).
 __device__ int list_pages(const MlaPagePool& p, bool live, int from, int to, int want, int32_t* ids, int* warp_tot) {
@@ -152,24 +174,21 @@ __device__ __forceinline__ void copy_rows(const MlaPagePool& to, const MlaPagePo
 __global__ void __launch_bounds__(kPlanThreads) k_fork_plan(const MlaPagePool p, const int32_t* __restrict__ src,
                                                             const int32_t* __restrict__ dst, int n) {
     __shared__ int warp_tot[kPlanThreads / 32];
+    __shared__ uint32_t seen[MLA_MAX_BATCH / 32];
+    __shared__ int32_t near_ids[kPlanThreads];  // the fresh pages, if they are few
     pdl_wait();
     pdl_trigger();
     const View v(p);
     auto in_range = [&](int b) { return b >= 0 && b < p.batch; };
-    // a destination named twice takes its last pair
-    for (int i = threadIdx.x; i < n; i += kPlanThreads)
-        if (in_range(dst[i])) v.owner[dst[i]] = -1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kPlanThreads)
-        if (in_range(dst[i])) atomicMax(&v.owner[dst[i]], i);
-    __syncthreads();
+    const bool twice = named_twice(p, dst, n, seen);  // a destination named twice takes its last pair
+    if (twice) last_named(p, dst, n, v.owner);
     int need = 0;
     for (int base = 0; base < n; base += kPlanThreads) {
         const int i = base + (int)threadIdx.x;
         int fresh = -2, rows = 0;
         if (i < n) {
             const int a = src[i], b = dst[i];
-            if (!in_range(a) || !in_range(b) || v.owner[b] != i) {
+            if (!in_range(a) || !in_range(b) || (twice && v.owner[b] != i)) {
                 record_error(sink(p), MLA_DEV_BAD_REQUEST);
             } else if (a != b) {
                 rows = p.seq_lens[a];
@@ -191,7 +210,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_fork_plan(const MlaPagePool p,
         }
         need += total;
     }
-    const int got = list_pages(p, false, 0, p.n_pages, need, v.ids, warp_tot);
+    int32_t* ids = need <= kPlanThreads ? near_ids : v.ids;
+    const int got = list_pages(p, false, 0, p.n_pages, need, ids, warp_tot);
     __syncthreads();  // ids complete
     if (threadIdx.x == 0) v.ctl[0] = got < need;
     if (got < need) {
@@ -200,7 +220,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_fork_plan(const MlaPagePool p,
     }
     for (int i = threadIdx.x; i < n; i += kPlanThreads) {
         if (v.fresh[i] < 0) continue;
-        const int page = v.ids[v.fresh[i]];
+        const int page = ids[v.fresh[i]];
         v.fresh[i] = page;
         p.refs[page] = 1;
     }
@@ -280,17 +300,12 @@ __global__ void __launch_bounds__(kCopyThreads) k_release(const MlaPagePool p, c
 __global__ void __launch_bounds__(kPlanThreads) k_reserve(const MlaPagePool p, const int32_t* __restrict__ requests,
                                                           int n, int tokens) {
     __shared__ int warp_tot[kPlanThreads / 32];
+    __shared__ uint32_t seen[MLA_MAX_BATCH / 32];
     const View v(p);
     auto request = [&](int i) { return requests ? requests[i] : i; };
     auto in_range = [&](int b) { return b >= 0 && b < p.batch; };
-    if (requests) {  // a request named twice gets its pages once
-        for (int i = threadIdx.x; i < n; i += kPlanThreads)
-            if (in_range(request(i))) v.owner[request(i)] = -1;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += kPlanThreads)
-            if (in_range(request(i))) atomicMax(&v.owner[request(i)], i);
-        __syncthreads();
-    }
+    const bool twice = requests && named_twice(p, requests, n, seen);  // then it gets its pages once
+    if (twice) last_named(p, requests, n, v.owner);
     int need = 0;
     for (int base = 0; base < n; base += kPlanThreads) {
         const int i = base + (int)threadIdx.x;
@@ -299,7 +314,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_reserve(const MlaPagePool p, c
             const int b = request(i);
             if (!in_range(b)) {
                 record_error(sink(p), MLA_DEV_BAD_REQUEST);
-            } else if (!requests || v.owner[b] == i) {
+            } else if (!twice || v.owner[b] == i) {
                 const int64_t want = ((int64_t)p.seq_lens[b] + tokens + kPage - 1) / kPage;
                 if (p.seq_lens[b] < 0 || want > p.max_blocks || p.held[b] < 0) record_error(sink(p), MLA_DEV_BAD_POSITION);
                 else more = max(0, (int)want - p.held[b]);
