@@ -226,7 +226,7 @@ class LayerStackGraph:
       library for batches up to 64), then `ffn(l, h)` if given (capturable torch ops that
       update h in place, e.g. the layer's FFN with its residual).
 
-    With advance=True the graph also adds 1 to every cache's seq_lens. Device errors of any
+    With advance=True the graph also adds 1 to every cache's seq_lens (once, if caches share it). Device errors of any
     layer are raised by replay() / synchronize() (each runner's pinned host error word).
     """
 
@@ -265,9 +265,9 @@ class LayerStackGraph:
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self._step()
-            if advance:
-                for c in self.caches:
-                    c.seq_lens.add_(1)
+            if advance:  # once each, where the layers share their row counts
+                for lens in {c.seq_lens.data_ptr(): c.seq_lens for c in self.caches}.values():
+                    lens.add_(1)
 
     def _params_warm(self) -> None:
         """Run each layer's library call once outside the capture (workspace allocation,

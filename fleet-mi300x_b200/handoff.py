@@ -39,6 +39,8 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     otherwise read back, which waits for the device.
     """
     dev = cache.device
+    if dev.type != "cuda" or rows.device != dev:
+        raise ValueError(f"rows and the cache must be on one GPU, got {rows.device} and {dev}")
     if rows.dtype != torch.bfloat16 or rows.dim() != 2 or rows.shape[1] < ROW or rows.stride(1) != 1:
         raise ValueError("rows must be bf16 [n, >= 576] with contiguous rows")
     starts = torch.as_tensor(row_start, dtype=torch.int64)
@@ -63,6 +65,9 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     if raw:
         if norm_w is None or cos is None or sin is None:
             raise ValueError("raw rows need norm_w, cos and sin")
+        if norm_w.dtype != torch.bfloat16 or cos.dtype != torch.float32 or sin.dtype != torch.float32 or not (
+                norm_w.device == cos.device == sin.device == dev):
+            raise ValueError("norm_w must be bf16, cos and sin f32, on the cache's device")
         r.kv_a_norm_w, r.rope_cos, r.rope_sin = _ptr(norm_w), _ptr(cos), _ptr(sin)
         r.max_pos, r.rms_eps = cos.shape[0], eps
     r.error_word = _ptr(error_word)

@@ -386,7 +386,53 @@ def test_refusals(cuda_device):
     with pytest.raises(ValueError):
         fleet.rows_to_pages(cache, torch.zeros(4, 576, device=dev), [0, 4])  # not bf16
     with pytest.raises(ValueError):
+        fleet.rows_to_pages(cache, torch.zeros(4, 576, dtype=BF), [0, 4])  # rows on the host
+    with pytest.raises(ValueError):
+        fleet.rows_to_pages(cache, torch.zeros(4, 576, dtype=BF, device=dev), [0, 5])
+    with pytest.raises(native.MlaError):
+        fleet.rows_to_pages(cache, torch.zeros(4, 576, dtype=BF, device=dev), [0, 4], total=-1)
+    with pytest.raises(ValueError):
         fleet.PagedLatentCache8.from_tensors(cache.pages[:, :100], cache.scales, cache.block_table, cache.seq_lens)
+
+
+def test_static_step(cuda_device):
+    """The step with the library's own workspace: the bits of the step with the caller's."""
+    st, cache, out = run8(cuda_device, [200, 9], 150)
+    got = torch.empty_like(out)
+    p = st.runner.params(st.q, st.kv_a, cache, got)
+    native.check(st.runner.lib.mla_decode_step_static(p, torch.cuda.current_stream().cuda_stream), "static", p)
+    torch.cuda.synchronize()
+    assert torch.equal(got, out)
+
+
+def test_uk_norms(cuda_device):
+    """The largest column norm of every head's W_UK: fp32 sums of 128 squares, then a root, 2^-16 relative at most."""
+    w = workloads.make_layer_weights(9).kv_b_proj
+    got = torch.empty(16, device=cuda_device)
+    lib = native.load_library()
+    kv_b = w.to(cuda_device)
+    assert lib.mla_uk_norms(kv_b.data_ptr(), got.data_ptr(), None) == 0
+    torch.cuda.synchronize()
+    want = w.double().view(16, 256, 512)[:, :128].norm(dim=1).amax(1)
+    assert ((got.cpu().double() - want).abs() <= want * 2.0 ** -16).all()
+    assert lib.mla_uk_norms(None, got.data_ptr(), None) == -1
+    assert lib.mla_uk_norms(kv_b.data_ptr() + 2, got.data_ptr(), None) == -3
+
+
+def test_zero_and_tiny_queries(cuda_device):
+    """A query of zeros attends evenly; one far below bf16's usual range keeps its values (the bounds follow
+    from the derivation in check_out: they scale with the scores)."""
+    st, cache, _ = run8(cuda_device, [100, 70], 160)
+    codes = [R.read_request(cache, b, n + 1) for b, n in enumerate(st.lens)]
+    values = []
+    for c, e in codes:
+        f = np.exp2(np.repeat(e.astype(np.float64), 16, 0))[:len(c)]
+        values.append(c * np.concatenate([np.repeat(f[:, :1], 512, 1), np.repeat(f[:, 1:], 64, 1)], 1))
+    for scale in (0.0, 1e-12):
+        st.q = (st.q.float() * scale).to(BF)
+        out = st.runner.attend(st.q, st.kv_a, cache, check="sync")
+        st.check(out, lambda b: values[b], f"scale {scale}")
+        st.q = torch.randn(2, 3072, generator=torch.Generator().manual_seed(161)).to(BF).to(cuda_device)
 
 
 def test_read_and_write_rows_helpers(cuda_device):

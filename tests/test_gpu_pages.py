@@ -370,3 +370,24 @@ def test_operations_in_a_graph(cuda_device):
     for x in range(3):
         n = int(a.seq_lens[x])
         assert torch.equal(a.read_rows(x, 0, n), b.read_rows(x, 0, n))
+
+
+@pytest.mark.parametrize("bits,window", [(8, 0), (8, 100), (16, 0)])
+def test_parallel_decode_example(cuda_device, bits, window):
+    """The example end to end: samples advance, half end, what is left holds the shared prompt and its own pages."""
+    import importlib
+    example = importlib.import_module("fleet-mi300x_b200.parallel_decode")
+    got = example.run(layers=3, prompt=150, samples=4, steps=40, window=window, sinks=4 if window else 0, bits=bits)
+    assert got["rows"][:2] == [190, 190] and got["pages_held"] < got["pages_unshared"] + 2
+    assert torch.isfinite(got["h"][:2].float()).all()
+
+
+def test_stack_with_shared_row_counts_advances_once(cuda_device):
+    st = Step(cuda_device, [10], 600, max_pos=64)
+    own = fleet.PagedLatentCache8.for_lengths([10], extra_tokens=5, device=cuda_device)
+    other = fleet.PagedLatentCache8(own.n_pages, 1, own.max_blocks, device=cuda_device)
+    caches = [own, fleet.PagedLatentCache8.from_tensors(other.pages, other.scales, own.block_table, own.seq_lens)]
+    stack = fleet.LayerStackGraph([st.runner] * 2, caches, mode="slice", advance=True)
+    stack.replay()
+    stack.synchronize()
+    assert own.seq_lens.tolist() == [11]
