@@ -120,17 +120,31 @@ __device__ __forceinline__ bool share_amax(const RowShare& x, float& ac, float& 
 }
 
 // A share under the exponents e_c, e_r into slot `slot` of a page. inf: it may hold an infinity.
+// The scaling is a bf16 multiply of both halves: a power of two in bf16's range, so it is exact, but
+// for results below 2^-126, which e4m3 rounds to zero anyway.
 __device__ __forceinline__ void store_share(uint8_t* page, int slot, const RowShare& x, bool inf, int e_c, int e_r,
                                             int lane) {
-    const float f = pow2i(-e_c), g = pow2i(-e_r);
-    auto value = [&](float v) { return inf ? nan_if_inf(v) : v; };
+    const __nv_bfloat162 f = __float2bfloat162_rn(pow2i(-e_c));
+    const float g = pow2i(-e_r);
     uint32_t w[4];
+    float lo = __bfloat162float(x.lo), hi = __bfloat162float(x.hi);
+    if (!inf) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        w[k] = e4m3x4(value(__low2float(x.c[2 * k])) * f, value(__high2float(x.c[2 * k])) * f,
-                      value(__low2float(x.c[2 * k + 1])) * f, value(__high2float(x.c[2 * k + 1])) * f);
+        for (int k = 0; k < 4; ++k) {
+            const __nv_bfloat162 a = __hmul2(x.c[2 * k], f), b = __hmul2(x.c[2 * k + 1], f);
+            w[k] = e4m3x4(__low2float(a), __high2float(a), __low2float(b), __high2float(b));
+        }
+    } else {
+        const float s = pow2i(-e_c);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w[k] = e4m3x4(nan_if_inf(__low2float(x.c[2 * k])) * s, nan_if_inf(__high2float(x.c[2 * k])) * s,
+                          nan_if_inf(__low2float(x.c[2 * k + 1])) * s, nan_if_inf(__high2float(x.c[2 * k + 1])) * s);
+        lo = nan_if_inf(lo);
+        hi = nan_if_inf(hi);
+    }
     *reinterpret_cast<uint4*>(page + slot * kLora + 16 * lane) = make_uint4(w[0], w[1], w[2], w[3]);
-    const uint32_t r = e4m3x2(value(__bfloat162float(x.lo)) * g, value(__bfloat162float(x.hi)) * g);
+    const uint32_t r = e4m3x2(lo * g, hi * g);
     uint8_t* rope = page + kPage8Rope + slot * kRope + lane;
     rope[0] = (uint8_t)r;
     rope[32] = (uint8_t)(r >> 8);
