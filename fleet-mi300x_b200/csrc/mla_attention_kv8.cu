@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
         tmem_relinquish();
     } else if (warp == 2 && lane == 0) {
         for (int i = 0; i < kSlots; ++i) {
-            mbar_init(&S.full[i], 1);
+            mbar_init(&S.full[i], 2);  // the copies, the exponents
             mbar_init(&S.empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
 
     if (warp == 0) {
         // ------------------------------------------------------------ producer
-        // A page's number is loaded two pages ahead and its exponents one page ahead, so that
-        // neither latency is on the path. Up to kEarly pages go out before the wait on K1, none that
+        // A page's number is loaded two pages ahead and its exponents one page ahead, so that neither
+        // latency is on the path; they join the page's barrier after its copies were issued. Up to kEarly pages go out before the wait on K1, none that
         // K1 appends to (and whose exponents it may raise).
         if (lane == 0) {
             struct Page { int id; bool appended; };
@@ -349,32 +349,34 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             auto page_of = [&]() -> Page {
                 if (la.first()) vis = visible(la.b);
                 const int k = vis.tile(la.index());
-                int id = p.block_table[(int64_t)la.b * p.max_blocks + k];
-                if (id < 0 || id >= p.n_pages) { record_error(err, MLA_DEV_BAD_PAGE); id = 0; }
-                return Page{id, fresh && k == (vis.rows - 1) / kPage};
+                return Page{p.block_table[(int64_t)la.b * p.max_blocks + k], fresh && k == (vis.rows - 1) / kPage};
             };
-            auto exps_of = [&](int id) { return reinterpret_cast<const uint64_t*>(p.kv_scales)[id]; };
+            auto page_ok = [&](int id) { return id >= 0 && id < p.n_pages; };
+            auto exps_of = [&](int id) { return reinterpret_cast<const uint64_t*>(p.kv_scales)[page_ok(id) ? id : 0]; };
             bool waited = !pre;
             Page p0 = page_of(), p1 = p0, p2 = p0;
             la.next();
             if (la.valid()) p1 = page_of();
-            uint64_t ex0 = exps_of(p0.id), ex1 = ex0;
-            bool early0 = !waited, early1 = early0;  // loaded before the wait
+            uint64_t ex0 = 0, ex1 = 0;
+            bool early0 = true, early1 = true;  // not loaded yet, or before the wait
             uint32_t i = 0;
             TileCursor at = cur;
             for (; at.valid(); at.next(), ++i) {
                 if (!waited && (i >= kEarly || p0.appended)) { pdl_wait(); MLA_TL_WAITED(1); waited = true; }
-                if (p0.appended && early0) ex0 = exps_of(p0.id);
+                const uint32_t sl = i % kSlots;
+                if (i >= kSlots && !wait(&S.empty[sl], (i / kSlots - 1) & 1)) break;
+                if (!page_ok(p0.id)) record_error(err, MLA_DEV_BAD_PAGE);
+                const int id = page_ok(p0.id) ? p0.id : 0;
+                mbar_arrive_expect_tx(&S.full[sl], kSlotC + kSlotR);
+                tma_load_5d(smem + kOffC + sl * kSlotC, &tmap_c, &S.full[sl], 0, 0, 0, 0, id, kCacheEvictFirst);
+                tma_load_3d(smem + kOffR + sl * kSlotR, &tmap_r, &S.full[sl], 0, 0, id, kCacheEvictFirst);
+                if (i == 0 || (p0.appended && early0)) ex0 = exps_of(id);
                 la.next();
                 if (la.valid()) p2 = page_of();
                 ex1 = exps_of(p1.id);
                 early1 = !waited;
-                const uint32_t sl = i % kSlots;
-                if (i >= kSlots && !wait(&S.empty[sl], (i / kSlots - 1) & 1)) break;
                 S.exps[sl] = ex0;
-                mbar_arrive_expect_tx(&S.full[sl], kSlotC + kSlotR);
-                tma_load_5d(smem + kOffC + sl * kSlotC, &tmap_c, &S.full[sl], 0, 0, 0, 0, p0.id, kCacheEvictFirst);
-                tma_load_3d(smem + kOffR + sl * kSlotR, &tmap_r, &S.full[sl], 0, 0, p0.id, kCacheEvictFirst);
+                mbar_arrive(&S.full[sl]);
                 p0 = p1; p1 = p2; ex0 = ex1; early0 = early1;
             }
             if (!waited) pdl_wait();
