@@ -293,7 +293,11 @@ __global__ void __launch_bounds__(kCopyThreads) k_release(const MlaPagePool p, c
         p.seq_lens[b] = 0;
     }
     __syncthreads();
-    for (int k = threadIdx.x; k < held_s; k += kCopyThreads) drop(p, p.block_table[(int64_t)b * p.max_blocks + k]);
+    for (int k = threadIdx.x; k < held_s; k += kCopyThreads) {
+        int32_t& e = p.block_table[(int64_t)b * p.max_blocks + k];
+        drop(p, e);
+        e = -1;  // the page may be another's soon: a step on this request, unless it reserves, is an error
+    }
 }
 
 // One CTA: pages for `tokens` more rows of every named request (requests = NULL: all).

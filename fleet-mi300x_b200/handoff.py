@@ -34,7 +34,8 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     rows: bf16 [total, >= 576] on the cache's device; row_start: [batch + 1] (host or
     device, int); first_pos: [batch] or None (= 0). raw=True takes kv_a rows and needs
     norm_w (kv_a_layernorm weight) and the YaRN tables cos/sin. Does not change seq_lens.
-    On a PagedLatentCache8 the rows are rounded to e4m3 under their blocks' scales.
+    On a PagedLatentCache8 the rows are rounded to e4m3 under their blocks' scales; a request's rows
+    go in ascending order there, as rows that follow in the same block of 16 do not keep their values.
     total: row_start's last entry, if the caller knows it; with a device row_start it is
     otherwise read back, which waits for the device.
     """

@@ -109,7 +109,9 @@ class PagePool:
         self._call("mla_pool_fork", check, _ptr(src), _ptr(dst), src.numel())
 
     def release(self, requests, *, check: bool | str = True) -> None:
-        """Let go of the requests' pages; they hold nothing and have no rows afterwards."""
+        """Let go of the requests' pages; they hold nothing and have no rows afterwards, and their
+        block-table entries are -1: a step on one of them, before pages are reserved for it, is an
+        error (MLA_DEV_BAD_PAGE) and stores no row."""
         requests = _ids(requests, self.device)
         self._call("mla_pool_release", check, _ptr(requests), requests.numel())
 

@@ -117,12 +117,14 @@ typedef enum {
 /* An 8-bit cache (ABI v7). A page is MLA_PAGE8_BYTES: the latent part [64][512], then the rotary part
  * [64][64], both e4m3. Every block of MLA_SCALE_BLOCK rows of a page has one power-of-two scale per
  * part, held as its exponent in kv_scales: value = e4m3 * 2^exponent, where the exponent is the smallest
- * one, at least MLA_SCALE_MIN_EXP, that brings the block's largest finite magnitude to at most 448 (powers of two, so
- * that storing a row and re-expressing a block are exact up to e4m3's own rounding). A row that
+ * one, at least MLA_SCALE_MIN_EXP, that brings the block's largest finite magnitude to at most 448 (powers
+ * of two, so that storing a row and re-expressing a block are exact up to e4m3's own rounding). A row that
  * joins a block whose scale is too small for it raises the scale, and the block's earlier rows are
- * held anew under it. Infinities and NaN are held as NaN. Its split-KV kernel keeps the scores and the output in tensor
- * memory (tcgen05.mma kind::f8f6f4): the absorbed query and the probabilities enter as pairs of e4m3
- * values, together about as precise as bf16. Not with MLA_FLAG_CHECK_KERNEL, _TCGEN05, _QC_HILO, _P_HILO. */
+ * held anew under it. Later rows are not: a request's rows are stored in ascending order, and a call that
+ * stores rows before others of the same block leaves those others undefined. Infinities and NaN are
+ * held as NaN. Its split-KV kernel keeps the scores and the output in tensor memory (tcgen05.mma
+ * kind::f8f6f4): the absorbed query and the probabilities enter as pairs of e4m3 values, together about
+ * as precise as bf16. Not with MLA_FLAG_CHECK_KERNEL, _TCGEN05, _QC_HILO, _P_HILO. */
 #define MLA_FLAG_KV8 0x80
 #define MLA_SCALE_BLOCK 16
 #define MLA_SCALE_MIN_EXP (-64)
@@ -393,7 +395,8 @@ int mla_pool_scratch_size(const MlaPagePool* p, uint64_t* bytes);
  * destination of another (beams reordered among themselves). The free pages are those before the call.
  * Too few: MLA_DEV_NO_PAGE and no change. A destination named twice takes its last pair. */
 int mla_pool_fork(const MlaPagePool* p, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
-/* The requests' pages lose a holder each; held = seq_lens = 0. */
+/* The requests' pages lose a holder each; held = seq_lens = 0, and the block-table entries become -1, so that
+ * a step on such a request reports MLA_DEV_BAD_PAGE until pages are reserved for it. */
 int mla_pool_release(const MlaPagePool* p, const int32_t* requests, int32_t n, void* stream);
 /* Free pages for every request that holds too few for seq_lens + tokens rows (requests = NULL: all of
  * the batch, n ignored). Too few in all: MLA_DEV_NO_PAGE and no change. */
@@ -402,8 +405,8 @@ int mla_pool_reserve(const MlaPagePool* p, const int32_t* requests, int32_t n, i
  * before L), block-table entries and counts with them. */
 int mla_pool_compact(const MlaPagePool* p, void* stream);
 /* Page src[i] of every layer of `from` into page dst[i] of `to` (the same layers and kind; they may be
- * one pool). No page may be named twice in dst, or in both lists of one pool. Uses pages, scales, n_layers, kv8, n_pages and the error
- * words of `to`; the other fields are not looked at. */
+ * one pool). No page may be named twice in dst, or in both lists of one pool. Uses pages, scales, n_layers,
+ * kv8, n_pages and the error words of `to`; the other fields are not looked at. */
 int mla_copy_pages(const MlaPagePool* to, const MlaPagePool* from, const int32_t* src, const int32_t* dst, int32_t n,
                    void* stream);
 

@@ -372,6 +372,34 @@ def test_operations_in_a_graph(cuda_device):
         assert torch.equal(a.read_rows(x, 0, n), b.read_rows(x, 0, n))
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_step_on_a_released_request_stores_nothing(cuda_device, bits):
+    """Its former page has gone to another request: the step reports the missing page and the new owner's
+    rows stay as they are; after a reservation the request starts over."""
+    dev = cuda_device
+    st = Step(dev, [64, 0], 520, max_pos=300)
+    cls = fleet.PagedLatentCache8 if bits == 8 else fleet.PagedLatentCache
+    cache = cls(6, 2, 4, device=dev)
+    pool = fleet.PagePool(cache)
+    cache.seq_lens[0] = 64
+    pool.reserve(1, [0])
+    pool.release([0], check="sync")
+    assert cache.block_table[0].tolist()[:2] == [-1, -1]
+    cache.seq_lens[1] = 64
+    pool.reserve(0, [1], check="sync")  # page 0, formerly request 0's
+    rows = random_rows(64, 521).to(dev)
+    fleet.rows_to_pages(cache, rows, [0, 0, 64])
+    before = cache.read_rows(1, 0, 64).clone()
+    pool.reserve(1, [1], check="sync")
+    with pytest.raises(native.MlaError) as e:
+        st.runner.attend(st.q, st.kv_a, cache, check="sync")
+    assert e.value.code == 1
+    assert torch.equal(cache.read_rows(1, 0, 64), before)
+    pool.reserve(1, [0], check="sync")
+    st.runner.attend(st.q, st.kv_a, cache, check="sync")
+    assert torch.equal(cache.read_rows(1, 0, 64), before)
+
+
 @pytest.mark.parametrize("bits,window", [(8, 0), (8, 100), (16, 0)])
 def test_parallel_decode_example(cuda_device, bits, window):
     """The example end to end: samples advance, half end, what is left holds the shared prompt and its own pages."""
