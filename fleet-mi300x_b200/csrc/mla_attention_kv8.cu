@@ -340,8 +340,9 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
     if (warp == 0) {
         // ------------------------------------------------------------ producer
         // A page's number is loaded two pages ahead and its exponents one page ahead, so that neither
-        // latency is on the path; they join the page's barrier after its copies were issued. Up to kEarly pages go out before the wait on K1, none that
-        // K1 appends to (and whose exponents it may raise).
+        // latency is on the path; they join the page's barrier after its copies were issued. Up to
+        // kEarly pages go out before the wait on K1, none that K1 appends to (and whose exponents it
+        // may raise).
         if (lane == 0) {
             struct Page { int id; bool appended; };
             TileCursor la = cur;  // two pages ahead of the one being loaded
@@ -398,14 +399,15 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             const uint32_t qb = cur.seg & 1, sb = j & 1;
             const int pages = cur.pages();
             const bool last = cur.last();
-            if (cur.first() && !wait(&S.q_full[qb], (cur.seg >> 1) & 1)) break;
-            if (j >= 2 && !wait(&S.p_full[sb], ((j - 2) >> 1) & 1)) break;  // the buffer's scores were read
+            ok = !cur.first() || wait(&S.q_full[qb], (cur.seg >> 1) & 1);
+            ok &= j < 2 || wait(&S.p_full[sb], ((j - 2) >> 1) & 1);  // the buffer's scores were read
             const uint64_t b = dqc + ((qb * kQ) >> 4), br = dqr + ((qb * kQ) >> 4);
             for (int k = 0; k < pages; ++k, ++i) {
                 const uint32_t sl = i % kSlots;
-                if (!(ok = wait(&S.full[sl], (i / kSlots) & 1))) break;
+                ok &= wait(&S.full[sl], (i / kSlots) & 1);
+                ok = __all_sync(0xffffffffu, ok);  // one answer for the warp, even if a wait ran out in some lanes
+                if (!ok) break;
                 tc_fence_after();
-                __syncwarp();
                 const uint64_t a = dc + ((sl * kSlotC) >> 4), ar = dr + ((sl * kSlotR) >> 4);
                 const uint32_t d = tmem + kTmemS + kTmemSSize * sb + kTmemSPage * k;
                 if (elect_one()) {
@@ -444,12 +446,12 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), pages, ks) << ks;
             const uint32_t sl0 = i % kSlots, sl1 = (i + 1) % kSlots;
-            if (!wait(&S.p_full[sb], (j >> 1) & 1)) break;
-            if (first && cur.seg >= 2 && !wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1)) break;
-            if (!wait(&S.full[sl0], (i / kSlots) & 1)) break;
-            if (pages > 1 && !wait(&S.full[sl1], ((i + 1) / kSlots) & 1)) break;
+            bool ok = wait(&S.p_full[sb], (j >> 1) & 1);
+            ok &= !first || cur.seg < 2 || wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1);
+            ok &= wait(&S.full[sl0], (i / kSlots) & 1);
+            ok &= pages < 2 || wait(&S.full[sl1], ((i + 1) / kSlots) & 1);
+            if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            __syncwarp();
             const uint64_t a0 = dc + ((sl0 * kSlotC) >> 4), a1 = dc + ((sl1 * kSlotC) >> 4), b = dp + ((sb * kP) >> 4);
             const uint32_t d = tmem + kTmemO + ob * kTmemOSize;
             if (elect_one()) {
