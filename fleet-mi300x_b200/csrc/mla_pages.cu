@@ -167,6 +167,11 @@ __device__ __forceinline__ void copy_rows(const MlaPagePool& to, const MlaPagePo
         static_cast<uint64_t*>(to.scales[layer])[dst] = static_cast<const uint64_t*>(from.scales[layer])[src];
 }
 
+// The last thing in a kernel that changes tables or counts of rows. A decode step's first kernel reads
+// those of its inputs before its own wait on the kernel before it, so they must not only be
+// written but have reached the L2 when this kernel's CTAs are gone; nor do these kernels signal early.
+__device__ __forceinline__ void tables_done() { __threadfence(); }
+
 // ---------------------------------------------------------------------------- fork
 // One CTA: which pairs take part, the rows of each, and the fresh page of each that
 // needs one (fresh[i] = page, -1 = none, -2 = the pair takes no part). ctl[0] = 1 if
@@ -278,6 +283,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_fork_switch(const MlaPagePool 
         p.held[b] = full + (fresh >= 0);
         p.seq_lens[b] = rows;
     }
+    tables_done();
 }
 
 // ---------------------------------------------------------------------------- release, reserve
@@ -298,6 +304,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_release(const MlaPagePool p, c
         drop(p, e);
         e = -1;  // the page may be another's soon: a step on this request, unless it reserves, is an error
     }
+    tables_done();
 }
 
 // One CTA: pages for `tokens` more rows of every named request (requests = NULL: all).
@@ -351,6 +358,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_reserve(const MlaPagePool p, c
         __syncwarp();  // held was read
         if ((threadIdx.x & 31) == 0) p.held[b] = held + more;
     }
+    tables_done();
 }
 
 // ---------------------------------------------------------------------------- compact
@@ -394,12 +402,14 @@ __global__ void __launch_bounds__(kCopyThreads) k_compact_tables(const MlaPagePo
         p.refs[v.ids[i]] = p.refs[v.ids2[i]];
         p.refs[v.ids2[i]] = 0;
     }
+    tables_done();
 }
 
 // ---------------------------------------------------------------------------- copy
 __global__ void __launch_bounds__(kCopyThreads) k_copy_pages(const MlaPagePool to, const MlaPagePool from,
                                                              const int32_t* __restrict__ src,
                                                              const int32_t* __restrict__ dst, int parts) {
+    pdl_wait();
     const int s = src[blockIdx.x], d = dst[blockIdx.x];
     if (s < 0 || s >= from.n_pages || d < 0 || d >= to.n_pages) {
         if (threadIdx.x == 0) record_error(ErrSink{to.error_word, to.error_host}, MLA_DEV_BAD_PAGE);
@@ -420,7 +430,6 @@ cudaError_t launch_pool_fork(const MlaPagePool& p, const int32_t* src, const int
     cudaError_t e = launch_pdl(k_fork_plan, dim3(1), dim3(kPlanThreads), 0, s, p, src, dst, n);
     if (e == cudaSuccess)
         e = launch_pdl(k_fork_share, dim3(n, 1 + p.n_layers), dim3(kCopyThreads), 0, s, p, src);
-    // The last kernel signals nothing early: a decode step that follows may read the tables before its own wait.
     if (e == cudaSuccess) e = launch_pdl(k_fork_switch, dim3(n), dim3(kCopyThreads), 0, s, p, dst);
     return e == cudaSuccess ? cudaGetLastError() : e;
 }
@@ -447,8 +456,7 @@ cudaError_t launch_copy_pages(const MlaPagePool& to, const MlaPagePool& from, co
     // few pages: several CTAs per page and layer, so that the copy still fills the GPU
     const int64_t jobs = (int64_t)n * to.n_layers;
     const int parts = jobs >= 4 * sm_count ? 1 : (jobs >= sm_count ? 3 : 9);
-    k_copy_pages<<<dim3(n, to.n_layers * parts), kCopyThreads, 0, s>>>(to, from, src, dst, parts);
-    return cudaGetLastError();
+    return launch_pdl(k_copy_pages, dim3(n, to.n_layers * parts), dim3(kCopyThreads), 0, s, to, from, src, dst, parts);
 }
 
 }  // namespace mla

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(kRowsThreads, raw ? 3 : 5) k_rows_to_pages8(co
     __shared__ alignas(16) float2 red[kRowsPerCta];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t v = blockIdx.x;
+    pdl_wait();
     // the request of this slot: largest b with block_slot(b) <= v, 32 probes per round
     int lo = 0, hi = r.batch;
     while (hi - lo > 1) {
@@ -187,10 +188,8 @@ cudaError_t launch_rows_to_pages(const MlaRowsToPages& r, int sm_count, cudaStre
         if (r.total_rows <= 0) return cudaSuccess;
         if (slots > INT32_MAX) return cudaErrorInvalidValue;
         if (r.mode == MLA_ROWS_RAW)
-            k_rows_to_pages8<true><<<(unsigned)slots, kRowsThreads, 0, stream>>>(r);
-        else
-            k_rows_to_pages8<false><<<(unsigned)slots, kRowsThreads, 0, stream>>>(r);
-        return cudaGetLastError();
+            return launch_pdl(k_rows_to_pages8<true>, dim3((unsigned)slots), dim3(kRowsThreads), 0, stream, r);
+        return launch_pdl(k_rows_to_pages8<false>, dim3((unsigned)slots), dim3(kRowsThreads), 0, stream, r);
     }
     const int64_t need = (r.total_rows + kRowsPerCta - 1) / kRowsPerCta;
     const int64_t cap = (int64_t)sm_count * 16;

@@ -39,29 +39,32 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     total: row_start's last entry, if the caller knows it; with a device row_start it is
     otherwise read back, which waits for the device.
     """
-    dev = cache.device
-    if dev.type != "cuda" or rows.device != dev:
+    pages, table = cache.pages, cache.block_table
+    dev = pages.device
+    if not pages.is_cuda or rows.device != dev:
         raise ValueError(f"rows and the cache must be on one GPU, got {rows.device} and {dev}")
-    if rows.dtype != torch.bfloat16 or rows.dim() != 2 or rows.shape[1] < ROW or rows.stride(1) != 1:
+    shape, stride = rows.shape, rows.stride()
+    if rows.dtype != torch.bfloat16 or len(shape) != 2 or shape[1] < ROW or stride[1] != 1:
         raise ValueError("rows must be bf16 [n, >= 576] with contiguous rows")
+    batch, max_blocks = table.shape
     starts = torch.as_tensor(row_start, dtype=torch.int64)
-    if starts.dim() != 1 or starts.numel() != cache.batch + 1:
-        raise ValueError(f"row_start needs batch + 1 = {cache.batch + 1} entries")
+    if starts.shape != (batch + 1,):
+        raise ValueError(f"row_start needs batch + 1 = {batch + 1} entries")
     if total is None:
         total = int(starts[-1].item())
     if starts.device != dev:
         starts = starts.to(dev)
-    if total > rows.shape[0]:
-        raise ValueError(f"row_start ends at {total} but only {rows.shape[0]} rows were given")
+    if total > shape[0]:
+        raise ValueError(f"row_start ends at {total} but only {shape[0]} rows were given")
     pos = None if first_pos is None else torch.as_tensor(first_pos, dtype=torch.int32, device=dev)
     r = native.new_rows()
     r.mode = native.ROWS_RAW if raw else native.ROWS_FINAL
-    r.batch = cache.batch
+    r.batch = batch
     r.total_rows = total
-    r.rows, r.rows_stride = _ptr(rows), rows.stride(0) if rows.shape[0] > 1 else rows.shape[1]
-    r.row_start, r.first_pos = _ptr(starts), _ptr(pos)
-    r.block_table, r.max_blocks, r.n_pages = _ptr(cache.block_table), cache.max_blocks, cache.n_pages
-    r.kv_cache = _ptr(cache.pages)
+    r.rows, r.rows_stride = rows.data_ptr(), stride[0] if shape[0] > 1 else shape[1]
+    r.row_start, r.first_pos = starts.data_ptr(), _ptr(pos)
+    r.block_table, r.max_blocks, r.n_pages = table.data_ptr(), max_blocks, pages.shape[0]
+    r.kv_cache = pages.data_ptr()
     r.kv_scales = _scales_ptr(cache)
     if raw:
         if norm_w is None or cos is None or sin is None:
@@ -72,7 +75,9 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
         r.kv_a_norm_w, r.rope_cos, r.rope_sin = _ptr(norm_w), _ptr(cos), _ptr(sin)
         r.max_pos, r.rms_eps = cos.shape[0], eps
     r.error_word = _ptr(error_word)
-    native.check(native.load_library().mla_rows_to_pages(r, _raw_stream(dev)), "mla_rows_to_pages")
+    code = native.load_library().mla_rows_to_pages(r, _raw_stream(dev))
+    if code:
+        native.check(code, "mla_rows_to_pages")
 
 
 def read_flat_cache(path: str | Path, layers: int, max_pos: int) -> torch.Tensor:
