@@ -13,9 +13,9 @@
 // per clock), so 128 tokens x 16 heads cost 36 + 16 MMAs, 1,570 of the about 3,300 clocks of
 // their HBM time. N is nearly free, so it carries precision: an operand
 // that is not 8 bits already enters as a pair of e4m3 values side by side on N,
-// x = hi + lo / 16, about as precise as bf16 (8 significant bits):
-//   scores  S^T[t][hi 16 | lo 16]  = C[t][:] . Q[hi | lo]   (latent and rotary apart: their scales differ)
-//   output  O^T[l][hi 16 | lo 16] += C^T[l][t] P^T[t][hi | lo]
+// x = hi + lo / 16, about as precise as bf16 (8 significant bits) for x in [2^-6, 448]:
+//   scores  S^T[t][hi 16 | lo 16] = C[t][:] . Q[hi | lo]   (latent and rotary apart: their scales differ)
+//   output  O^T[l][n]            += C^T[l][t] P^T[t][n],  n = hi 16 | lo 16 of P', then of 2^14 P'
 // The same tile bytes are the K-major A operand of the scores and the MN-major A
 // operand of the output.
 //
@@ -24,7 +24,14 @@
 // P'_t 2^-ec_t. P' lies in [0, 256]; a typical largest one is 16, so that a
 // later score may exceed the reference 16-fold before the output is rescaled (the
 // rescale reads and writes O in tensor memory, which happens in the first few tiles
-// of a segment only). Sums, scores and the output are fp32.
+// of a segment only). A pair of P' alone would end at 2^-14: many rows behind a dominant one,
+// as behind an attention sink, would leave the output and still count in the row sum. So a
+// P' below 2^-6 is held as the pair of 2^14 P' instead, in 32 columns of its own: 8
+// significant bits down to P' = 2^-20, 2^-24 of a typical largest one, fewer below, none
+// below 2^-28. The wider N costs an output MMA 8 clocks on 40, and shared memory and tensor
+// memory have room for one P and one output instead of two of each (256 x 4096: K2 106.3 us, 104.2
+// without).
+// Sums, scores and the output are fp32.
 //
 // Pages (the plan's units) are TMA'd into a ring of five; a tile is up to two pages of a request. The
 // scores are M = 64 MMAs per page, so that a page needs no neighbour in the ring and its scores start
@@ -37,8 +44,8 @@
 //   2      output MMAs
 //   3      loads the query of the next segment: K1 left it as the operand's image
 //   4-11   softmax: one token and eight heads per thread
-//   12-15  partials of a finished segment, while the next one runs (its output has the other half of
-//          the tensor memory; written by the softmax warps, a boundary cost about 2.3 us)
+//   12-15  partials of a finished segment, while the next one's first scores run (written by the
+//          softmax warps, a boundary cost about 2.3 us)
 // The MMA warps run their loops as whole warps and elect a lane for the MMAs, so that
 // descriptors stay in uniform registers: issued from a lane-0 branch, an MMA took 60-70
 // clocks of moving them there.
@@ -64,14 +71,16 @@ constexpr int kGroup = 8 * kLora;               // 4096: 8 rows of the latent pa
 constexpr int kSlotC = kPage * kLora;           // 32,768
 constexpr int kSlotR = kPage * kRope;           // 4,096
 constexpr int kN = kQ8N;                        // hi | lo
+constexpr int kNP = 2 * kN;                     // of P', then of 2^14 P'
 constexpr int kQ = kQ8C + kQ8R;                 // a request's query image
-constexpr int kP = kTok * kN;                   // [128 tokens][32 B]
+constexpr int kP = kTok * kNP;                  // [128 tokens][64 B]
+constexpr float kPSmall = 0x1p-6f, kPShift = 0x1p14f;  // P' below the first is held as kPShift P'
 
 constexpr int kOffC = 0;
 constexpr int kOffR = kOffC + kSlots * kSlotC;
 constexpr int kOffQ = kOffR + kSlots * kSlotR;
 constexpr int kOffP = kOffQ + 2 * kQ;
-constexpr int kOffMisc = kOffP + 2 * kP;
+constexpr int kOffMisc = kOffP + kP;
 
 struct Smem {
     uint64_t full[kSlots], empty[kSlots];
@@ -92,10 +101,11 @@ constexpr int kSmemBytes = kOffMisc + (int)sizeof(Smem) + 1024;  // + alignment 
 static_assert(kSmemBytes <= 232448, "K2 (8-bit) shared memory exceeds 227 KB");
 static_assert(kOffP % 1024 == 0 && kOffQ % 1024 == 0 && kQ % 1024 == 0, "operands must stay 1024-byte aligned");
 
-// Tensor memory columns: two score buffers (per page of the tile: latent 32 | rotary 32), two outputs of four
-// blocks of 32. The scores of a page (M = 64) lie in lanes 0-15 of each warp's 32.
+// Tensor memory columns: two score buffers (per page of the tile: latent 32 | rotary 32), an output of four
+// blocks of 64. The scores of a page (M = 64) lie in lanes 0-15 of each warp's 32.
 constexpr int kTmemS = 0, kTmemSPage = 2 * kN, kTmemSSize = 2 * kTmemSPage;
-constexpr int kTmemO = 2 * kTmemSSize, kTmemOSize = 4 * kN, kTmemCols = 512;
+constexpr int kTmemO = 2 * kTmemSSize, kTmemCols = 512;
+static_assert(kTmemO + 4 * kNP == kTmemCols, "the tensor memory is full");
 
 // Instruction descriptor of kind::f8f6f4 with e4m3 A/B and fp32 D (the fields of
 // idesc_bf16_f32; format 0 = e4m3).
@@ -104,7 +114,7 @@ __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N, int a_mn_major, 
            (uint32_t(M >> 4) << 24);
 }
 constexpr uint32_t kIdescQK = idesc_e4m3(64, kN, 0, 0);
-constexpr uint32_t kIdescPV = idesc_e4m3(128, kN, 1, 1);
+constexpr uint32_t kIdescPV = idesc_e4m3(128, kNP, 1, 1);
 
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                        uint32_t accumulate) {
@@ -117,9 +127,9 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_
 }
 
 // Shared-memory descriptor as smem_desc_sw128, with the layout (swizzle) given: 2 =
-// 128-byte, 4 = 64-byte, 6 = 32-byte; sbo: bytes between groups of 8 rows (K-major)
+// 128-byte, 4 = 64-byte; sbo: bytes between groups of 8 rows (K-major)
 // or of 8 k (MN-major).
-constexpr int kSw128 = 2, kSw64 = 4, kSw32 = 6;
+constexpr int kSw128 = 2, kSw64 = 4;
 __device__ __forceinline__ uint64_t desc_of(uint32_t saddr, uint32_t sbo_bytes, int layout) {
     return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(1) << 16) | (uint64_t((sbo_bytes >> 4) & 0x3FFF) << 32) |
            (uint64_t(1) << 46) | (uint64_t(layout) << 61);
@@ -434,7 +444,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
     } else if (warp == 2) {
         // ------------------------------------------------------------ output MMAs
         const uint64_t dc = desc_of(smem_u32(smem + kOffC), kGroup, kSw128);
-        const uint64_t dp = desc_of(smem_u32(smem + kOffP), 8 * kN, kSw32);
+        const uint64_t dp = desc_of(smem_u32(smem + kOffP), 8 * kNP, kSw64);
         Visible vis;
         uint32_t j = 0, i = 0;
         for (; cur.valid(); i += cur.pages(), cur.next(), ++j) {
@@ -447,13 +457,13 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             for (int ks = 0; ks < 4; ++ks) on |= (uint32_t)step_on(vis, cur.index(), pages, ks) << ks;
             const uint32_t sl0 = i % kSlots, sl1 = (i + 1) % kSlots;
             bool ok = wait(&S.p_full[sb], (j >> 1) & 1);
-            ok &= !first || cur.seg < 2 || wait(&S.o_empty[ob], ((cur.seg >> 1) - 1) & 1);
+            ok &= !first || cur.seg < 1 || wait(&S.o_empty[ob ^ 1], ((cur.seg - 1) >> 1) & 1);
             ok &= wait(&S.full[sl0], (i / kSlots) & 1);
             ok &= pages < 2 || wait(&S.full[sl1], ((i + 1) / kSlots) & 1);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            const uint64_t a0 = dc + ((sl0 * kSlotC) >> 4), a1 = dc + ((sl1 * kSlotC) >> 4), b = dp + ((sb * kP) >> 4);
-            const uint32_t d = tmem + kTmemO + ob * kTmemOSize;
+            const uint64_t a0 = dc + ((sl0 * kSlotC) >> 4), a1 = dc + ((sl1 * kSlotC) >> 4);
+            const uint32_t d = tmem + kTmemO;
             if (elect_one()) {
                 uint32_t acc = first ? 0u : 1u;
 #pragma unroll
@@ -462,7 +472,7 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                         const uint64_t a = (ks < 2 ? a0 : a1) + (((ks & 1) * 4 * kGroup) >> 4);
 #pragma unroll
                         for (int cb = 0; cb < 4; ++cb)
-                            mma_f8(d + kN * cb, a + ((cb * 1024) >> 4), b + ((ks * 32 * kN) >> 4), kIdescPV, acc);
+                            mma_f8(d + kNP * cb, a + ((cb * 1024) >> 4), dp + ((ks * 32 * kNP) >> 4), kIdescPV, acc);
                         acc = 1u;
                     }
                     if (ks == 1) tc_commit(&S.empty[sl0]);
@@ -519,15 +529,18 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             float* acc = part_acc + part * kHeads * kLora + 32 * sp + lane;
 #pragma unroll 2
             for (int k = 0; k < 8; ++k) {  // four blocks, two halves of the heads
-                float o[kHh], q[kHh];
-                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + ob * kTmemOSize + kN * (k >> 1) + kHh * (k & 1));
+                float o[kHh], q[kHh], so[kHh], sq[kHh];
+                const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + kNP * (k >> 1) + kHh * (k & 1));
                 tmem_ld8(ta, o);
                 tmem_ld8(ta + kHeads, q);
+                tmem_ld8(ta + kN, so);
+                tmem_ld8(ta + kN + kHeads, sq);
                 tmem_wait_ld();
-                loaded(o); loaded(q);
+                loaded(o); loaded(q); loaded(so); loaded(sq);
 #pragma unroll
                 for (int h = 0; h < kHh; ++h)
-                    acc[(kHh * (k & 1) + h) * kLora + 128 * (k >> 1)] = fmaf(q[h], 0.0625f, o[h]);
+                    acc[(kHh * (k & 1) + h) * kLora + 128 * (k >> 1)] =
+                        fmaf(fmaf(sq[h], 0.0625f, so[h]), 1.f / kPShift, fmaf(q[h], 0.0625f, o[h]));
             }
             tc_fence_before();
             __syncwarp();
@@ -621,9 +634,9 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
                     tc_fence_after();
                     __syncwarp();
 #pragma unroll 2
-                    for (int k = 0; k < 8; ++k) {  // four blocks, hi and lo
+                    for (int k = 0; k < 4 * kNP / kHeads; ++k) {  // four blocks of two pairs
                         float o[kHh];
-                        const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + (cur.seg & 1) * kTmemOSize + 16 * k + h0);
+                        const uint32_t ta = tmem_lane_addr(tmem, sp, kTmemO + kHeads * k + h0);
                         tmem_ld8(ta, o);
                         tmem_wait_ld();
                         loaded(o);
@@ -636,27 +649,32 @@ __global__ void __launch_bounds__(kv8::kThreads, 1)
             }
             // ---- P' as e4m3 pairs, the row sums over the unrounded values ----
             const float back = pow2i(-(int)ex.x);
-            uint32_t hi[2], lo[2];
+            uint32_t hi[2], lo[2], small[2];  // four heads each; small: 0xFF where the pair is of 2^14 P'
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 uint32_t x[2], y[2];
+                small[k] = 0;
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int h = 4 * k + 2 * i;
-                    const float u = sees ? fast_exp2(s[h] - m[h]) : 0.f, w = sees ? fast_exp2(s[h + 1] - m[h + 1]) : 0.f;
+                    float u = sees ? fast_exp2(s[h] - m[h]) : 0.f, w = sees ? fast_exp2(s[h + 1] - m[h + 1]) : 0.f;
                     l[h] = fmaf(u, back, l[h]);
                     l[h + 1] = fmaf(w, back, l[h + 1]);
+                    if (u < kPSmall) { u *= kPShift; small[k] |= 0xFFu << (16 * i); }
+                    if (w < kPSmall) { w *= kPShift; small[k] |= 0xFF00u << (16 * i); }
                     e4m3_pairs(u, w, x[i], y[i]);
                 }
                 hi[k] = x[0] | (x[1] << 16);
                 lo[k] = y[0] | (y[1] << 16);
             }
-            if (j >= 2) wait(&S.pv_done[sb], ((j - 2) >> 1) & 1);  // the P buffer is free
+            if (j >= 1) wait(&S.pv_done[(j - 1) & 1], ((j - 1) >> 1) & 1);  // the last tile's P was read
             {
-                uint8_t* pt = smem + kOffP + sb * kP + tok * kN + h0;
-                const int sw = (tok >> 2) & 1;
-                *reinterpret_cast<uint2*>(pt + (sw << 4)) = make_uint2(hi[0], hi[1]);
-                *reinterpret_cast<uint2*>(pt + ((sw ^ 1) << 4)) = make_uint2(lo[0], lo[1]);
+                uint8_t* pt = smem + kOffP + tok * kNP + h0;
+                const int sw = (tok >> 1) & 3;
+                *reinterpret_cast<uint2*>(pt + (sw << 4)) = make_uint2(hi[0] & ~small[0], hi[1] & ~small[1]);
+                *reinterpret_cast<uint2*>(pt + ((sw ^ 1) << 4)) = make_uint2(lo[0] & ~small[0], lo[1] & ~small[1]);
+                *reinterpret_cast<uint2*>(pt + ((sw ^ 2) << 4)) = make_uint2(hi[0] & small[0], hi[1] & small[1]);
+                *reinterpret_cast<uint2*>(pt + ((sw ^ 3) << 4)) = make_uint2(lo[0] & small[0], lo[1] & small[1]);
             }
             if (!sees && !dry && step_on(vis, index, pages, 2 * half + (slot >> 5))) {  // 0 * stale bytes must be 0
                 uint8_t* row = smem + kOffC + sl * kSlotC + (slot >> 3) * kGroup + (slot & 7) * 128 + (h0 >> 3) * 2048;

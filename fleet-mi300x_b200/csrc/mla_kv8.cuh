@@ -62,7 +62,8 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 }
 
 // Two values, |values| <= 448 or NaN, as a pair of e4m3 values each: x = hi + lo / 16 to about 2^-9 of
-// x (its own rounding to f16 on the way is 2^-12). hi and lo hold both values, the first in the low byte.
+// x for |x| >= 2^-6 (its own rounding to f16 on the way is 2^-12), to 2^-14 for smaller ones. hi and lo hold
+// both values, the first in the low byte.
 __device__ __forceinline__ void e4m3_pairs(float x0, float x1, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x0, x1);
     hi = __nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(h), __NV_SATFINITE, __NV_E4M3);

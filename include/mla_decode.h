@@ -124,7 +124,9 @@ typedef enum {
  * stores rows before others of the same block leaves those others undefined. Infinities and NaN are
  * held as NaN. Its split-KV kernel keeps the scores and the output in tensor memory (tcgen05.mma
  * kind::f8f6f4): the absorbed query and the probabilities enter as pairs of e4m3 values, together about
- * as precise as bf16. Not with MLA_FLAG_CHECK_KERNEL, _TCGEN05, _QC_HILO, _P_HILO. */
+ * as precise as bf16. Unlike bf16 they have a floor: a probability keeps 8 bits down to about 2^-24 of a
+ * segment's largest p * 2^exponent and counts in the output down to 2^-32 of it; the floor of a query element is
+ * 2^-22 of a bound of its head's largest. Not with MLA_FLAG_CHECK_KERNEL, _TCGEN05, _QC_HILO, _P_HILO. */
 #define MLA_FLAG_KV8 0x80
 #define MLA_SCALE_BLOCK 16
 #define MLA_SCALE_MIN_EXP (-64)
