@@ -135,11 +135,34 @@ class MlaDecodeAttention:
                         "prologue": self.lib.mla_prologue, "attention": self.lib.mla_attention,
                         "merge": self.lib.mla_merge_uv, "combine": self.lib.mla_exchange_combine}
         self._ws: torch.Tensor | None = None
-        # the column norms of W_UK, from which a step on an 8-bit cache knows its query's scale
-        self.uk_norm = torch.empty(cfg.heads, dtype=torch.float32, device=dev)
-        native.check(self.lib.mla_uk_norms(_ptr(self.kv_b), _ptr(self.uk_norm), _raw_stream(dev)), "mla_uk_norms")
+        # the column norms of W_UK, from which a step on an 8-bit cache knows its query's scale, and
+        # (the tensor, its version, its address) that they are of
+        self.uk_norm: torch.Tensor | None = None
+        self._norm_of: tuple | None = None
         self._step_key: tuple | None = None   # attend(): params of the last call, reused for the same tensors
         self._step_p: native.MlaDecodeParams | None = None
+
+    # ------------------------------------------------------------------ norms of W_UK (8-bit caches)
+    def update_norms(self, kv_b: torch.Tensor | None = None) -> None:
+        """Take the column norms of W_UK anew, on the current stream.
+
+        Every step on an 8-bit cache, and every replay of a graph of this package, does so where `kv_b` is
+        another tensor than before or has changed in place by torch's version counter (a tensor made in
+        inference mode has none: then at every step). Call it after a change that torch does not count
+        (through .data, or by a kernel of one's own), and after any change before replaying a
+        graph that one captured oneself."""
+        kv_b = self.kv_b if kv_b is None else kv_b
+        if self.uk_norm is None:
+            self.uk_norm = torch.empty(self.cfg.heads, dtype=torch.float32, device=self.device)
+        native.check(self.lib.mla_uk_norms(_ptr(kv_b), _ptr(self.uk_norm), _raw_stream(self.device)), "mla_uk_norms")
+        # in a capture nothing has run yet
+        self._norm_of = None if kv_b.is_inference() or torch.cuda.is_current_stream_capturing() else (
+            weakref.ref(kv_b), kv_b._version, kv_b.data_ptr())
+
+    def _keep_norms(self, kv_b: torch.Tensor) -> None:
+        of = self._norm_of
+        if of is None or of[0]() is not kv_b or of[1] != kv_b._version or of[2] != kv_b.data_ptr():
+            self.update_norms(kv_b)
 
     # ------------------------------------------------------------------ params
     def params(self, q: torch.Tensor | None, kv_a: torch.Tensor | None, cache: PagedLatentCache,
@@ -178,6 +201,7 @@ class MlaDecodeAttention:
         p.num_ctas = self.num_ctas
         p.flags = self.flags | (0 if new_row else native.FLAG_NO_NEW_ROW)
         if isinstance(cache, PagedLatentCache8):
+            self._keep_norms(self.kv_b)
             p.flags |= native.FLAG_KV8
             p.kv_scales = _ptr(cache.scales)
             p.uk_norm = _ptr(self.uk_norm)
@@ -253,8 +277,11 @@ class MlaDecodeAttention:
             p = self.params(q, kv_a, cache, out, rope_pos=rope_pos, shard_out=shard_out, new_row=new_row,
                             exchange=exchange)
             self._step_key, self._step_p = key, p
-        elif out is not None:
-            p.out, p.out_stride = out.data_ptr(), _row_stride(out)
+        else:
+            if p.kv_scales:
+                self._keep_norms(self.kv_b)
+            if out is not None:
+                p.out, p.out_stride = out.data_ptr(), _row_stride(out)
         code = self._stages[stage](p, _raw_stream(self.device))
         if code:
             native.check(code, f"mla {stage}", p)
@@ -278,6 +305,8 @@ class MlaDecodeAttention:
         if key != self._step_key or self._ws is None or p.workspace != self._ws.data_ptr():
             p = self.params(None, None, cache, out, x_n=x_n)
             self._step_key, self._step_p = key, p
+        elif p.kv_scales:
+            self._keep_norms(self.kv_b)
         code = self._stages[stage](p, _raw_stream(self.device))
         if code:
             native.check(code, f"mla {stage}", p)

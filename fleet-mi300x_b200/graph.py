@@ -22,7 +22,15 @@ from __future__ import annotations
 import torch
 
 from .attention import MlaDecodeAttention
-from .cache import PagedLatentCache
+from .cache import PagedLatentCache, PagedLatentCache8
+
+
+def _norm_sources(runners, caches) -> list:
+    """(runner, kv_b) of the captured steps on 8-bit caches whose kv_b may change between replays: the
+    query's scale has to follow it (MlaDecodeAttention.update_norms). A kv_b made in inference mode has its
+    norms taken inside the capture."""
+    return [(r, r.kv_b) for r, c in zip(runners, caches)
+            if isinstance(c, PagedLatentCache8) and not r.kv_b.is_inference()]
 
 
 class DecodeGraph:
@@ -63,6 +71,7 @@ class DecodeGraph:
             self._step()
             if advance:
                 cache.seq_lens.add_(1)
+        self._norms = _norm_sources([runner], [cache])
 
     def _step(self) -> None:
         if self.inputs == "x_n":
@@ -74,6 +83,8 @@ class DecodeGraph:
         """Run the captured step on the current stream; returns `out`. Raises first if
         an earlier step recorded a device error."""
         self.runner.raise_pending()
+        for r, kv_b in self._norms:
+            r._keep_norms(kv_b)
         self.graph.replay()
         return self.out
 
@@ -177,6 +188,7 @@ class HostStepGraph:
             self._step()
             if advance:
                 cache.seq_lens.add_(1)
+        self._norms = _norm_sources([runner], [cache])
 
     def _step(self) -> None:
         self.x_dev.copy_(self.x_host, non_blocking=True)
@@ -188,6 +200,8 @@ class HostStepGraph:
         stream has reached this point). Raises first if an earlier step recorded a
         device error."""
         self.runner.raise_pending()
+        for r, kv_b in self._norms:
+            r._keep_norms(kv_b)
         self.graph.replay()
         return self.out_host
 
@@ -268,6 +282,7 @@ class LayerStackGraph:
             if advance:  # once each, where the layers share their row counts
                 for lens in {c.seq_lens.data_ptr(): c.seq_lens for c in self.caches}.values():
                     lens.add_(1)
+        self._norms = _norm_sources(self.runners, self.caches)
 
     def _params_warm(self) -> None:
         """Run each layer's library call once outside the capture (workspace allocation,
@@ -298,6 +313,8 @@ class LayerStackGraph:
         """Run the captured step on the current stream (raises first if an earlier step of
         any layer recorded a device error)."""
         self._raise_pending()
+        for r, kv_b in self._norms:
+            r._keep_norms(kv_b)
         self.graph.replay()
 
     def synchronize(self) -> None:

@@ -231,7 +231,8 @@ typedef struct MlaDecodeParams {
     void* kv_scales;  /* MLA_FLAG_KV8: int8 [n_pages][4][2], the exponents of each 16-row block of a page
                          (latent part, rotary part), 8-byte aligned; else NULL */
     const float* uk_norm; /* MLA_FLAG_KV8: f32 [16], per head the largest 2-norm of a column of W_UK
-                         (mla_uk_norms; a property of kv_b, made once with the weights); else NULL */
+                         (mla_uk_norms), of kv_b as it is when the step runs: take them anew whenever kv_b
+                         changes, or a larger query saturates unnoticed; else NULL */
     int32_t window;   /* sliding window: the query sees the last `window` rows, its own among them; 0 = all.
                          Only the pages that hold a visible row are read. Default and MLA_FLAG_KV8 kernels;
                          not with a sequence-sharded step (MLA_FLAG_NO_NEW_ROW, shard_out, world). */
@@ -356,7 +357,8 @@ void mla_rows_init(MlaRowsToPages* r);
 int mla_rows_to_pages(const MlaRowsToPages* r, void* stream);
 
 /* norms[h] = max_l |W_UK[h][:, l]|_2 of a layer's kv_b (16 floats, device memory): what a step on an
- * 8-bit cache takes as uk_norm, to know the scale of its absorbed query ahead of it. Run once per layer. */
+ * 8-bit cache takes as uk_norm, to know the scale of its absorbed query ahead of it. Run once per layer, and
+ * again after every change of kv_b. */
 int mla_uk_norms(const void* kv_b, float* norms, void* stream);
 
 /* The life of cache pages (ABI v7): fork, release, reserve, compact and copy, for the caches of
