@@ -263,7 +263,8 @@ __device__ __forceinline__ void drop(const MlaPagePool& p, int page) {
     }
 }
 
-// Pair x: the destination lets go of its old pages and takes over.
+// Pair x: the destination lets go of its old pages and takes over. Entries past its new pages
+// are emptied, as release does: their pages may be another's soon.
 __global__ void __launch_bounds__(kCopyThreads) k_fork_switch(const MlaPagePool p, const int32_t* __restrict__ dst) {
     pdl_wait();
     const View v(p);
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kCopyThreads) k_fork_switch(const MlaPagePool 
     const int old = min(p.held[b], p.max_blocks);
     for (int k = threadIdx.x; k < max(old, full); k += kCopyThreads) {
         if (k < old) drop(p, row[k]);
-        if (k < full) row[k] = keep[k];
+        row[k] = k < full ? keep[k] : -1;
     }
     __syncthreads();  // held and the entry at `full` were read
     if (threadIdx.x == 0) {

@@ -101,7 +101,8 @@ class PagePool:
     def fork(self, src, dst, *, check: bool | str = True) -> None:
         """Request dst[i] becomes a copy of request src[i] as it was before the call, for all i at once:
         it shares the full pages and gets its own copy of the rows of a last page that is not
-        full. Its former pages are let go of. src[i] == dst[i] changes nothing; a request may
+        full. Its former pages, reserved ones among them, are let go of, and entries past its new ones are -1, as after
+        release. src[i] == dst[i] changes nothing; a request may
         be both a source and a destination. Too few free pages: nothing changes, MLA_DEV_NO_PAGE."""
         src, dst = _ids(src, self.device), _ids(dst, self.device)
         if src.numel() != dst.numel():

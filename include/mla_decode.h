@@ -397,7 +397,8 @@ int mla_pool_scratch_size(const MlaPagePool* p, uint64_t* bytes);
  * before the call: the full pages are shared, the rows of a last page that is not full are copied
  * into a free page. src[i] == dst[i] changes nothing; a request may be source of some pairs and
  * destination of another (beams reordered among themselves). The free pages are those before the call.
- * Too few: MLA_DEV_NO_PAGE and no change. A destination named twice takes its last pair. */
+ * Too few: MLA_DEV_NO_PAGE and no change. A destination named twice takes its last pair. Entries of a
+ * destination past its new pages, up to those it held, become -1 (see mla_pool_release). */
 int mla_pool_fork(const MlaPagePool* p, const int32_t* src, const int32_t* dst, int32_t n, void* stream);
 /* The requests' pages lose a holder each; held = seq_lens = 0, and the block-table entries become -1, so that
  * a step on such a request reports MLA_DEV_BAD_PAGE until pages are reserved for it. */

@@ -419,3 +419,32 @@ def test_stack_with_shared_row_counts_advances_once(cuda_device):
     stack.replay()
     stack.synchronize()
     assert own.seq_lens.tolist() == [11]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_step_past_a_fork_without_a_page_stores_nothing(cuda_device, bits):
+    """A destination that had more pages than it gets: the step that needs another page, not reserved,
+    reports it, and the rows of the request that its former page went to stay as they are."""
+    dev = cuda_device
+    st = Step(dev, [64, 64, 64], 530, max_pos=300)
+    cls = fleet.PagedLatentCache8 if bits == 8 else fleet.PagedLatentCache
+    cache = cls(6, 3, 4, device=dev)
+    pool = fleet.PagePool(cache)
+    cache.seq_lens.copy_(torch.tensor([64, 130, 0], dtype=torch.int32))
+    pool.reserve(0)                       # request 0 page 0, request 1 pages 1, 2, 3
+    rows = random_rows(64, 531).to(dev)
+    fleet.rows_to_pages(cache, rows, [0, 64, 64, 64])
+    pool.fork([0], [1], check="sync")     # request 1 shares page 0; pages 1, 2, 3 are free
+    assert cache.block_table[1].tolist() == [0, -1, -1, 0]
+    cache.seq_lens[2] = 128
+    pool.reserve(0, [2], check="sync")    # pages 1 and 2, formerly request 1's
+    fleet.rows_to_pages(cache, random_rows(128, 532).to(dev), [0, 0, 0, 128])
+    before = cache.read_rows(2, 0, 128).clone()
+    pool.reserve(1, [0, 2], check="sync")
+    with pytest.raises(native.MlaError) as e:
+        st.runner.attend(st.q, st.kv_a, cache, check="sync")
+    assert e.value.code == 1
+    assert torch.equal(cache.read_rows(2, 0, 128), before)
+    pool.reserve(1, [1], check="sync")
+    st.runner.attend(st.q, st.kv_a, cache, check="sync")
+    assert torch.equal(cache.read_rows(2, 0, 128), before)
