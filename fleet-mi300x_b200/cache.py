@@ -117,7 +117,8 @@ class PagedLatentCache8(PagedLatentCache):
     [64][64], both e4m3. `scales` is int8 [n_pages, 4, 2]: per block of 16 rows the exponents of the
     power-of-two scales of the two parts, value = e4m3 * 2**exponent. An exponent is the smallest
     one, at least -64, that brings the block's largest finite magnitude to at most 448; a row that joins a
-    started block may raise it, and the block's earlier rows are then held anew under it.
+    started block may raise it, and the block's earlier rows are then held anew under it (a row that is
+    stored again in its place, as by a repeated step, leaves the raised one).
     Infinities and NaN are held as NaN. Rows are stored by the decode step
     (MlaDecodeAttention) and by rows_to_pages; both take this class as they take
     PagedLatentCache. Pages that two requests share (PagePool.fork) must not be appended to.

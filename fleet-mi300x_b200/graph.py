@@ -23,6 +23,7 @@ import torch
 
 from .attention import MlaDecodeAttention
 from .cache import PagedLatentCache, PagedLatentCache8
+from .native import PAGE_SIZE
 
 
 def _norm_sources(runners, caches) -> list:
@@ -33,6 +34,28 @@ def _norm_sources(runners, caches) -> list:
             if isinstance(c, PagedLatentCache8) and not r.kv_b.is_inference()]
 
 
+def _warm(step, caches, dev: torch.device) -> None:
+    """Run `step` once outside the capture, on a side stream (library set-up, workspaces, cuBLAS state). Its
+    rows go into each request's next slot, which the first replay writes again; but a row that joins a
+    started block of an 8-bit cache also raises the block's scale and rounds the earlier rows under it, so the
+    pages that those rows go to are put back."""
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        kept = []
+        for c in caches:
+            if isinstance(c, PagedLatentCache8):
+                block = c.seq_lens.long() // PAGE_SIZE
+                page = c.block_table.gather(1, block.clamp(0, c.max_blocks - 1)[:, None])[:, 0].long()
+                page = page[(block >= 0) & (block < c.max_blocks) & (page >= 0) & (page < c.n_pages)]
+                kept.append((c, page, c.pages[page], c.scales[page]))
+        step()
+        for c, page, pages, scales in kept:
+            c.pages[page], c.scales[page] = pages, scales
+    torch.cuda.current_stream(dev).wait_stream(side)
+    torch.cuda.synchronize(dev)
+
+
 class DecodeGraph:
     """`runner`'s step over `cache` captured as a CUDA graph.
 
@@ -40,7 +63,7 @@ class DecodeGraph:
     inputs="qkv": the step from q [B, 3072] and kv_a [B, 576] (K1-K3 only).
     Set-up runs the step once eagerly on a side stream (library set-up, workspace,
     cuBLAS state), which writes a row into each request's next slot; the first
-    replay writes that slot again.
+    replay writes that slot again. The pages of an 8-bit cache are as before it.
     """
 
     def __init__(self, runner: MlaDecodeAttention, cache: PagedLatentCache, *, inputs: str = "x_n",
@@ -60,12 +83,7 @@ class DecodeGraph:
                                                                   device=dev)
         self.out = out if out is not None else torch.empty(B, cfg.heads * cfg.v_head, dtype=bf, device=dev)
 
-        side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):
-            self._step()
-        torch.cuda.current_stream(dev).wait_stream(side)
-        torch.cuda.synchronize(dev)
+        _warm(self._step, [cache], dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self._step()
@@ -177,12 +195,7 @@ class HostStepGraph:
         self.out_host = torch.empty(B, cfg.heads * cfg.v_head, dtype=bf).pin_memory()
         self.x_dev = torch.zeros(B, cfg.hidden, dtype=bf, device=dev)
         self.out_dev = torch.empty(B, cfg.heads * cfg.v_head, dtype=bf, device=dev)
-        side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):
-            self._step()
-        torch.cuda.current_stream(dev).wait_stream(side)
-        torch.cuda.synchronize(dev)
+        _warm(self._step, [cache], dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self._step()
@@ -270,12 +283,7 @@ class LayerStackGraph:
             self.h = h if h is not None else torch.zeros(B, cfg.hidden, dtype=bf, device=dev)
             self.x_n = torch.empty(B, cfg.hidden, dtype=bf, device=dev)
             self.attn = torch.empty(B, cfg.heads * cfg.v_head, dtype=bf, device=dev)
-        side = torch.cuda.Stream(dev)
-        side.wait_stream(torch.cuda.current_stream(dev))
-        with torch.cuda.stream(side):  # library set-up and workspaces before the capture
-            self._params_warm()
-        torch.cuda.current_stream(dev).wait_stream(side)
-        torch.cuda.synchronize(dev)
+        _warm(self._params_warm, self.caches, dev)
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph):
             self._step()

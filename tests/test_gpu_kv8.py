@@ -444,3 +444,30 @@ def test_read_and_write_rows_helpers(cuda_device):
     want.write(0, rows.double().numpy())
     got = cache.read_rows(0, 0, 37)
     assert got.dtype == torch.float32 and np.array_equal(got.double().cpu().numpy(), want.values(37))
+
+
+@pytest.mark.parametrize("kind", ["decode", "stack"])
+def test_setting_up_a_graph_leaves_the_rows_alone(cuda_device, kind):
+    """The set-up's step stores a row of whatever the buffers hold; a large one must not coarsen the started
+    block's earlier rows for good. The first replay equals the eager step on an untouched cache."""
+    lens = [37, 64, 5]
+    st = Step(cuda_device, lens, 170)
+    a, b = (make_cache(lens, cuda_device, 171) for _ in range(2))
+    for cache in (a, b):
+        fill(cache, lens, 172)
+    before = a.pages.clone(), a.scales.clone()
+    want = st.runner.attend(st.q, st.kv_a, b, check="sync").clone()
+    q, kv = torch.randn_like(st.q), torch.randn_like(st.kv_a) * 1e6
+    if kind == "decode":
+        graph = fleet.DecodeGraph(st.runner, a, inputs="qkv", q=q, kv_a=kv)
+    else:
+        graph = fleet.LayerStackGraph([st.runner], [a], mode="slice", q=[q], kv_a=[kv])
+    assert torch.equal(a.pages, before[0]) and torch.equal(a.scales, before[1])
+    q.copy_(st.q)
+    kv.copy_(st.kv_a)
+    out = graph.replay()
+    graph.synchronize()
+    assert torch.equal(out if kind == "decode" else graph.out[0], want)
+    for r, n in enumerate(lens):
+        assert np.array_equal(R.read_request(a, r, n + 1)[1], R.read_request(b, r, n + 1)[1])
+        assert np.array_equal(R.read_request(a, r, n + 1)[0], R.read_request(b, r, n + 1)[0])
