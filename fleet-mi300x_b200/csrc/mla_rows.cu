@@ -27,7 +27,8 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages(const MlaRowsToP
     const int lane = threadIdx.x & 31;
     const __nv_bfloat16* rows = reinterpret_cast<const __nv_bfloat16*>(r.rows);
     __nv_bfloat16* cache = reinterpret_cast<__nv_bfloat16*>(r.kv_cache);
-    for (int64_t i = (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5); i < r.total_rows;
+    const int64_t n = min(r.total_rows, r.row_start[r.batch]);  // rows past the last request's are nobody's
+    for (int64_t i = (int64_t)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5); i < n;
          i += (int64_t)gridDim.x * kRowsPerCta) {
         // request of row i: largest b with row_start[b] <= i
         int lo = 0, hi = r.batch;

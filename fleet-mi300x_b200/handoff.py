@@ -37,7 +37,7 @@ def rows_to_pages(cache: PagedLatentCache, rows: torch.Tensor, row_start, first_
     On a PagedLatentCache8 the rows are rounded to e4m3 under their blocks' scales; a request's rows
     go in ascending order there, as rows that follow in the same block of 16 do not keep their values.
     total: row_start's last entry, if the caller knows it; with a device row_start it is
-    otherwise read back, which waits for the device.
+    otherwise read back, which waits for the device. Rows from row_start's last entry on are not stored.
     """
     pages, table = cache.pages, cache.block_table
     dev = pages.device

@@ -116,3 +116,16 @@ def test_bad_positions_and_pages_are_reported(cuda_device):
     handoff.rows_to_pages(cache, rows, [0, 10, 20], [0, 0], error_word=err)
     torch.cuda.synchronize()
     assert int(err.item()) == 1  # MLA_DEV_BAD_PAGE
+
+
+def test_rows_past_the_last_start_are_not_stored(cuda_device):
+    """total= says how many rows the caller believes there are; rows that row_start gives to no request stay
+    out of the cache, on both caches."""
+    g = torch.Generator().manual_seed(77)
+    rows = torch.randn(40, 576, generator=g).to(torch.bfloat16).to(cuda_device)
+    starts = torch.tensor([0, 5, 30], device=cuda_device)
+    for cls in (fleet.PagedLatentCache, fleet.PagedLatentCache8):
+        a, b = (cls.for_lengths([60, 100], device=cuda_device, permute=False) for _ in range(2))
+        fleet.rows_to_pages(a, rows, starts, total=30)
+        fleet.rows_to_pages(b, rows, starts, total=40)
+        assert torch.equal(a.pages, b.pages)
