@@ -148,11 +148,17 @@ class PagedLatentCache8(PagedLatentCache):
 
     def write_rows(self, b: int, start: int, rows: torch.Tensor) -> None:
         """Store rows [n, 576] as request b's logical rows start..start+n-1 (on the GPU only:
-        the rounding and the blocks' scales are the library's)."""
+        the rounding and the blocks' scales are the library's). Waits for the device; rows without a place in
+        the block table or a page of the pool raise MlaError."""
         from .handoff import rows_to_pages
+        from .native import MlaError
         one = PagedLatentCache8.from_tensors(self.pages, self.scales, self.block_table[b:b + 1],
                                              self.seq_lens[b:b + 1])
-        rows_to_pages(one, rows.to(device=self.device, dtype=torch.bfloat16).contiguous(), [0, rows.shape[0]], [start])
+        word = torch.zeros(1, dtype=torch.int32, device=self.device)
+        rows_to_pages(one, rows.to(device=self.device, dtype=torch.bfloat16).contiguous(), [0, rows.shape[0]], [start],
+                      error_word=word)
+        if int(word):
+            raise MlaError(int(word), "device (write_rows)")
 
     def read_rows(self, b: int, start: int, n: int) -> torch.Tensor:
         """The values of request b's logical rows start..start+n-1, [n, 576] f32."""

@@ -471,3 +471,16 @@ def test_setting_up_a_graph_leaves_the_rows_alone(cuda_device, kind):
     for r, n in enumerate(lens):
         assert np.array_equal(R.read_request(a, r, n + 1)[1], R.read_request(b, r, n + 1)[1])
         assert np.array_equal(R.read_request(a, r, n + 1)[0], R.read_request(b, r, n + 1)[0])
+
+
+def test_write_rows_reports_rows_it_cannot_store(cuda_device):
+    cache = make_cache([70, 10], cuda_device, 180)
+    before = cache.pages.clone()
+    with pytest.raises(native.MlaError) as e:
+        cache.write_rows(1, 130, random_rows(20, 181))  # past the block table
+    assert e.value.code == 2
+    cache.block_table[0, 1] = cache.n_pages
+    with pytest.raises(native.MlaError) as e:
+        cache.write_rows(0, 64, random_rows(5, 182))
+    assert e.value.code == 1
+    assert torch.equal(cache.pages, before)
