@@ -10,9 +10,12 @@ operations together, as a server uses them.
   2. the other samples become copies of request 0 (PagePool.fork): shared full pages;
   3. every step reserves a page where a sample needs one, then replays one CUDA graph of all
      layers' attention blocks (LayerStackGraph, mode "block"), which appends and attends;
-  4. half the samples end early (release), and the pool is compacted.
+  4. half the samples end early (release), the pool is compacted, and a second graph, over the first
+     entries of the block table and the row counts, decodes the others to the end: a released request has
+     no page to store a row in, so a graph that steps it would report that.
 
-It prints the time per step, the pages held and what the samples would hold without sharing.
+It prints the time per step, the pages held at the end and what the samples that are left would hold
+without sharing.
 """
 from __future__ import annotations
 
@@ -61,22 +64,28 @@ def run(layers: int = 27, prompt: int = 4000, samples: int = 8, steps: int = 64,
         rows_to_pages(cache, kv_a, starts, raw=True, norm_w=runner.norm_w, cos=cos, sin=sin)
     pool.fork([0] * (samples - 1), range(1, samples))
 
+    live = samples if samples == 1 else samples // 2  # that decode to the end
     pool.reserve(1)
     h0 = torch.randn(samples, cfg.hidden, generator=g, device=dev).to(torch.bfloat16)
     norms = [torch.ones(cfg.hidden, dtype=torch.bfloat16, device=dev)] * layers
-    stack = LayerStackGraph(runners, caches, mode="block", h=h0.clone(), in_norms=norms, advance=True)
+    kw = dict(mode="block", in_norms=norms, advance=True)
+    stack = LayerStackGraph(runners, caches, h=h0, **kw)
+    some = [PagedLatentCache8.from_tensors(c.pages, c.scales, table[:live], lens[:live]) if bits == 8 else
+            PagedLatentCache.from_tensors(c.pages, table[:live], lens[:live]) for c in caches]
+    rest = stack if live == samples else LayerStackGraph(runners, some, h=h0[:live], **kw)
+    decoding, left = None, torch.arange(live, dtype=torch.int32, device=dev)  # None: every request
     begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
     begin.record()
     for step in range(steps):
-        if step == steps // 2 and samples > 1:
-            pool.release(range(samples // 2, samples))
+        if step == steps // 2 and live < samples:
+            pool.release(range(live, samples))
             pool.compact()
-        pool.reserve(1)
+            stack, decoding = rest, left
+        pool.reserve(1, decoding)
         stack.replay()
     end.record()
     stack.synchronize()
     pool.raise_pending()
-    live = samples if samples == 1 else samples // 2
     return {
         "layers": layers, "prompt": prompt, "samples": samples, "steps": steps, "window": window, "sinks": sinks,
         "bits": bits, "us_per_step": begin.elapsed_time(end) * 1e3 / steps, "pages_held": n_pages - pool.free_pages(),

@@ -448,3 +448,16 @@ def test_a_step_past_a_fork_without_a_page_stores_nothing(cuda_device, bits):
     pool.reserve(1, [1], check="sync")
     st.runner.attend(st.q, st.kv_a, cache, check="sync")
     assert torch.equal(cache.read_rows(2, 0, 128), before)
+
+
+def test_the_example_releases_half_of_its_samples(cuda_device):
+    """What it prints: the released samples have no rows and hold no pages afterwards, the others
+    share the prompt's full pages and have one of their own."""
+    import importlib
+    example = importlib.import_module("fleet-mi300x_b200.parallel_decode")
+    got = example.run(layers=2, prompt=150, samples=4, steps=40)
+    assert got["rows"] == [190, 190, 0, 0]
+    assert got["pages_held"] == 2 + 2 and got["pages_unshared"] == 2 * 3
+    assert got["h"].shape[0] == 2
+    got = example.run(layers=2, prompt=150, samples=1, steps=10)
+    assert got["rows"] == [160] and got["pages_held"] == 3
