@@ -167,11 +167,6 @@ __device__ __forceinline__ void copy_rows(const MlaPagePool& to, const MlaPagePo
         static_cast<uint64_t*>(to.scales[layer])[dst] = static_cast<const uint64_t*>(from.scales[layer])[src];
 }
 
-// The last thing in a kernel that changes tables or counts of rows. A decode step's first kernel reads
-// those of its inputs before its own wait on the kernel before it, so they must not only be
-// written but have reached the L2 when this kernel's CTAs are gone; nor do these kernels signal early.
-__device__ __forceinline__ void tables_done() { __threadfence(); }
-
 // ---------------------------------------------------------------------------- fork
 // One CTA: which pairs take part, the rows of each, and the fresh page of each that
 // needs one (fresh[i] = page, -1 = none, -2 = the pair takes no part). ctl[0] = 1 if
@@ -284,7 +279,6 @@ __global__ void __launch_bounds__(kCopyThreads) k_fork_switch(const MlaPagePool 
         p.held[b] = full + (fresh >= 0);
         p.seq_lens[b] = rows;
     }
-    tables_done();
 }
 
 // ---------------------------------------------------------------------------- release, reserve
@@ -305,7 +299,6 @@ __global__ void __launch_bounds__(kCopyThreads) k_release(const MlaPagePool p, c
         drop(p, e);
         e = -1;  // the page may be another's soon: a step on this request, unless it reserves, is an error
     }
-    tables_done();
 }
 
 // One CTA: pages for `tokens` more rows of every named request (requests = NULL: all).
@@ -359,7 +352,6 @@ __global__ void __launch_bounds__(kPlanThreads) k_reserve(const MlaPagePool p, c
         __syncwarp();  // held was read
         if ((threadIdx.x & 31) == 0) p.held[b] = held + more;
     }
-    tables_done();
 }
 
 // ---------------------------------------------------------------------------- compact
@@ -403,7 +395,6 @@ __global__ void __launch_bounds__(kCopyThreads) k_compact_tables(const MlaPagePo
         p.refs[v.ids[i]] = p.refs[v.ids2[i]];
         p.refs[v.ids2[i]] = 0;
     }
-    tables_done();
 }
 
 // ---------------------------------------------------------------------------- copy

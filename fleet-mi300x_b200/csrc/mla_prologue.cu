@@ -124,12 +124,14 @@ __device__ void plan_entries(const MlaDecodeParams& p, const int32_t* cum, const
     }
 }
 
-// The per-request warp's inputs that no earlier kernel writes: the row count and RoPE
-// position, the RoPE table rows of that position, the block-table entry of the new
-// row and kv_a_layernorm's weight. They are loaded before the wait on the previous
-// kernel (positions, tables and weights are the step's inputs, as for the split
-// plan that K2 derives before its own wait), so that after the wait only q_pe and
-// the raw kv_a row, the previous kernel's output, remain to be loaded.
+// The per-request warp's small inputs: the row count and RoPE position, the RoPE table
+// rows of that position, the block-table entry of the new row and kv_a_layernorm's
+// weight. They are loaded before the wait on the previous kernel, so that after the
+// wait only q_pe and the raw kv_a row, the previous kernel's output, remain to be
+// loaded. The weight and the RoPE tables no kernel writes; the counts and the table entry one may
+// (the caller's advance of seq_lens, a page operation), and what it wrote is sure to be seen
+// only after the wait: they are read again beside q_pe, past the L1, and all is loaded
+// anew if one differs. K2 and K3 start when every CTA of this kernel is past its wait.
 struct RowPre {
     int pos, rp, page;
     bool ok, append;
@@ -138,8 +140,8 @@ struct RowPre {
 };
 
 __device__ void request_rows_pre(const MlaDecodeParams& p, int b, int lane, RowPre& r) {
-    r.pos = p.seq_lens[b];
-    r.rp = p.rope_pos ? p.rope_pos[b] : r.pos;
+    r.pos = __ldcg(p.seq_lens + b);
+    r.rp = p.rope_pos ? __ldcg(p.rope_pos + b) : r.pos;
     r.append = new_row_count(p) != 0;
     const __nv_bfloat16* gam = reinterpret_cast<const __nv_bfloat16*>(p.kv_a_norm_w);
     if (r.append) {
@@ -158,15 +160,16 @@ __device__ void request_rows_pre(const MlaDecodeParams& p, int b, int lane, RowP
     const float* cs = p.rope_cos + (int64_t)r.rp * kRope;
     const float* sn = p.rope_sin + (int64_t)r.rp * kRope;
     r.c0 = cs[lane]; r.c1 = cs[32 + lane]; r.s0 = sn[lane]; r.s1 = sn[32 + lane];
-    if (r.append) r.page = p.block_table[(int64_t)b * p.max_blocks + r.pos / kPage];
+    if (r.append) r.page = __ldcg(p.block_table + (int64_t)b * p.max_blocks + r.pos / kPage);
 }
 
 // One warp, after the wait: q_pe RoPE of request b, then (unless the call stores no
 // row) kv_post + the cache append at local row seq_lens[b].
 template <bool kKv8>
 __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, float* q_scale, int b, int lane,
-                             const RowPre& r) {
-    if (!r.ok) return;
+                             RowPre& r) {
+    const int pos = __ldcg(p.seq_lens + b), rp = p.rope_pos ? __ldcg(p.rope_pos + b) : pos;
+    const int page = r.ok && r.append ? __ldcg(p.block_table + (int64_t)b * p.max_blocks + r.pos / kPage) : 0;
     const __nv_bfloat16* q = reinterpret_cast<const __nv_bfloat16*>(p.q) + (int64_t)b * p.q_stride;
     __nv_bfloat162 xq[kHeads];
 #pragma unroll
@@ -178,6 +181,8 @@ __device__ void request_rows(const MlaDecodeParams& p, __nv_bfloat16* qa, float*
 #pragma unroll
         for (int k = 0; k < 16; ++k) kin.gw[k] = r.gw[k];
     }
+    if (pos != r.pos || rp != r.rp || page != r.page) request_rows_pre(p, b, lane, r);
+    if (!r.ok) return;
 
     // q_pe of all 16 heads: lane j rotates pair j
     __nv_bfloat16* qrow = qa + (int64_t)b * kQRows * kRow;

@@ -484,3 +484,25 @@ def test_write_rows_reports_rows_it_cannot_store(cuda_device):
         cache.write_rows(0, 64, random_rows(5, 182))
     assert e.value.code == 1
     assert torch.equal(cache.pages, before)
+
+
+@pytest.mark.parametrize("bits,batch", [(8, 3), (16, 3), (16, 70)])
+def test_counts_changed_right_before_a_step(cuda_device, bits, batch):
+    """Row counts written by the kernel in front of the step (advance), many steps without a wait: every row at its
+    position, outputs as with a wait between."""
+    steps = 200
+    st = Step(cuda_device, [0] * batch, 190, max_pos=steps + 8)
+    cls = fleet.PagedLatentCache8 if bits == 8 else fleet.PagedLatentCache
+    a, b = (cls.for_lengths([0] * batch, extra_tokens=steps, permute=False, device=cuda_device) for _ in range(2))
+    g = torch.Generator().manual_seed(191)
+    kv = torch.randn(steps, batch, 576, generator=g).to(BF).to(cuda_device)
+    got, want = (torch.empty(steps, batch, 2048, dtype=BF, device=cuda_device) for _ in range(2))
+    for k in range(steps):
+        st.runner.attend(st.q, kv[k], a, got[k])
+        a.advance()
+    for k in range(steps):
+        st.runner.attend(st.q, kv[k], b, want[k], check="sync")
+        b.advance()
+        torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    assert torch.equal(a.pages, b.pages)
