@@ -96,7 +96,7 @@ __device__ __forceinline__ void rescale_rows(uint8_t* page, int blk, int n, floa
 
 // One lane's share of a bf16 row: 16 latent columns 16 lane .., rotary columns lane and 32 + lane.
 struct RowShare {
-    __nv_bfloat162 c[8];
+    alignas(16) __nv_bfloat162 c[8];  // loaded 16 bytes at a time
     __nv_bfloat16 lo, hi;
 };
 
