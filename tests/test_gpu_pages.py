@@ -461,3 +461,107 @@ def test_the_example_releases_half_of_its_samples(cuda_device):
     assert got["h"].shape[0] == 2
     got = example.run(layers=2, prompt=150, samples=1, steps=10)
     assert got["rows"] == [160] and got["pages_held"] == 3
+
+
+def last_named(ids):
+    """Each request once, where it is named last."""
+    return [b for i, b in enumerate(ids) if b not in ids[i + 1:]]
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_operations_on_requests_named_twice(cuda_device, bits):
+    """A destination named twice takes its last pair, beside the error; release acts once, and reserve
+    gives pages once, where a request is named last."""
+    t = Twin(cuda_device, bits, 2, 8, 61, 6, [0, 1, 63, 64, 65, 128, 200, 17])
+    r = random.Random(bits)
+    twice = {"fork": 0, "release": 0, "reserve": 0}
+    for step in range(24):
+        op = ("fork", "reserve", "fork", "release")[step % 4]
+        ids = [r.randrange(8) for _ in range(8 if op == "fork" else 5)]
+        twice[op] += len(set(ids)) < len(ids)
+        if op == "fork":
+            src = [r.randrange(8) for _ in ids]
+            enough = t.m.fork(src, ids)
+            if len(set(ids)) < len(ids) or not enough:
+                with pytest.raises(native.MlaError) as e:
+                    t.pool.fork(src, ids, check="sync")
+                assert e.value.code == (6 if len(set(ids)) < len(ids) else 5)
+            else:
+                t.pool.fork(src, ids, check="sync")
+        elif op == "release":
+            ids = ids[:2] + ids[:1]
+            t.m.release(ids)
+            t.pool.release(ids, check="sync")
+        else:
+            n = r.randint(0, 100)
+            if t.m.reserve(n, last_named(ids)):
+                t.pool.reserve(n, ids, check="sync")
+        t.check()
+    assert all(twice.values())
+
+
+def test_many_pairs_named_twice(cuda_device):
+    """More pairs than the planner's threads, each destination named twice, far apart and next to itself."""
+    batch, n_pages = 3000, 10000
+    g = torch.Generator().manual_seed(7)
+    lens = torch.randint(0, 130, (batch,), generator=g).to(torch.int32)
+    table = torch.arange(2 * batch, dtype=torch.int32).view(batch, 2).clone()
+    cache = fleet.PagedLatentCache8(n_pages, batch, 2, device=cuda_device)
+    lens.clamp_(max=128)
+    cache.block_table.copy_(table)
+    cache.seq_lens.copy_(lens)
+    pool = fleet.PagePool(cache)
+    free = torch.nonzero(pool.refs == 0)[:, 0].tolist()
+    dst = torch.cat([torch.randperm(batch // 2, generator=g), torch.randperm(batch // 2, generator=g)]).to(torch.int32)
+    dst[1::2][:500] = dst[0::2][:500]
+    src = torch.randint(0, batch, (batch,), generator=g).to(torch.int32)
+    with pytest.raises(native.MlaError) as e:
+        pool.fork(src.to(cuda_device), dst.to(cuda_device), check="sync")
+    assert e.value.code == 6
+    last = {int(b): i for i, b in enumerate(dst)}
+    want_lens, at = lens.tolist(), 0
+    want = [table[b, :-(-int(lens[b]) // 64)].tolist() for b in range(batch)]
+    new = {}
+    for i in range(batch):
+        a, b = int(src[i]), int(dst[i])
+        if last[b] != i or a == b:
+            continue
+        full, part = divmod(int(lens[a]), 64)
+        new[b] = table[a, :full].tolist() + ([free[at]] if part else [])
+        at += part > 0
+        want_lens[b] = int(lens[a])
+    for b, t in new.items():
+        want[b] = t
+    got, held = cache.block_table.tolist(), pool.held.tolist()
+    assert cache.seq_lens.tolist() == want_lens
+    assert [got[b][:held[b]] for b in range(batch)] == want
+    refs = torch.bincount(torch.tensor([p for t in want for p in t]), minlength=n_pages)
+    assert pool.refs.tolist() == refs.tolist()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_shared_pages_give_the_bits_of_pages_of_ones_own(cuda_device, bits):
+    """Four samples that share their prompt's full pages, and four that hold copies of them, in the same batch and
+    so on the same split: equal outputs and rows, bit for bit."""
+    dev, n0, steps = cuda_device, 150, 20
+    st = Step(dev, [n0], 540, max_pos=400)
+    cls = fleet.PagedLatentCache8 if bits == 8 else fleet.PagedLatentCache
+    cache = cls(40, 4, 8, device=dev)
+    pool = fleet.PagePool(cache)
+    prompt = random_rows(n0, 541).to(dev)
+    cache.seq_lens[0] = n0
+    pool.reserve(0, [0])
+    fleet.rows_to_pages(cache, prompt, [0] + [n0] * 4)
+    pool.fork([0, 0, 0], [1, 2, 3])
+    own = cls.for_lengths([n0] * 4, extra_tokens=steps, device=dev)
+    fleet.rows_to_pages(own, prompt.repeat(4, 1), [n0 * b for b in range(5)])
+    g = torch.Generator().manual_seed(542)
+    for step in range(steps):
+        q = torch.randn(4, 3072, generator=g).to(BF).to(dev)
+        kv = torch.randn(4, 576, generator=g).to(BF).to(dev)
+        pool.reserve(1)
+        assert torch.equal(st.runner.attend(q, kv, cache, check="sync"), st.runner.attend(q, kv, own, check="sync")), step
+        cache.advance()
+        own.advance()
+    for b in range(4):
+        assert torch.equal(cache.read_rows(b, 0, n0 + steps), own.read_rows(b, 0, n0 + steps))

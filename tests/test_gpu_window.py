@@ -126,3 +126,28 @@ def test_window_refusals(cuda_device):
         r.attend(st.q, st.kv_a, cache, shard_out=part)
     with pytest.raises(native.MlaError):
         r.attend(st.q, st.kv_a, cache, new_row=False)
+
+
+@pytest.mark.parametrize("window,sinks", [(150, 20), (1000, 1)])
+def test_the_hilo_forms_sharpen_a_window_too(cuda_device, window, sinks):
+    """qc_hilo and p_hilo together under a window, against the 64-bit value. What is left is the output's
+    rounding to bf16, as large as that of the 64-bit value itself (its 2-norm over 6,144 elements, to 5 %), and errors of
+    about 2^-16 in q_c, the probabilities and fp32 sums, held to 2^-12 in all. The default form has bf16's
+    rounding of q_c and of the probabilities besides and lies above that bound."""
+    lens = [700, 90, 1500]
+    st, cache, out = run16(cuda_device, lens, 380, window, sinks)
+    r = fleet.MlaDecodeAttention(CFG, st.runner.w, st.cos, st.sin, window=window, sinks=sinks, qc_hilo=True, p_hilo=True)
+    got = r.attend(st.q, st.kv_a, cache, check="sync").double().cpu().numpy()
+    out = out.double().cpu().numpy()
+    cos, sin = st.cos.double().cpu().numpy(), st.sin.double().cpu().numpy()
+    off, plain, rounding, norm = 0.0, 0.0, 0.0, 0.0
+    for b, n in enumerate(lens):
+        rows = np.concatenate([cache.read_rows(b, 0, n).double().cpu().numpy(), st.new_row(b)])
+        want = R.attention(st.q[b].double().cpu().numpy(), rows[R.visible(n, window, sinks)], st.kv_b, cos[n], sin[n],
+                           CFG.softmax_scale)[0]
+        off += ((got[b] - want) ** 2).sum()
+        plain += ((out[b] - want) ** 2).sum()
+        rounding += ((R.bf16(want) - want) ** 2).sum()
+        norm += (want ** 2).sum()
+    bound = 1.05 * rounding ** 0.5 + 2.0 ** -12 * norm ** 0.5
+    assert off ** 0.5 <= bound < plain ** 0.5, (np.sqrt(off / norm), bound / norm ** 0.5, np.sqrt(plain / norm))
