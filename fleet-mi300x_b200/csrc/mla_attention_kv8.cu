@@ -10,8 +10,8 @@
 // the SM has half the time per row (25 clocks at the copy peak), and m16n8k16 would
 // spend 70 % of its issue on it before a single conversion. An f8f6f4 MMA of K = 32 bytes and
 // N = 32 takes 40 clocks at M = 128 and 26 at M = 64 (measured: its shared-memory reads at 128 B
-// per clock), so 128 tokens x 16 heads cost 36 + 16 MMAs, 1,570 of the about 3,300 clocks of
-// their HBM time. N is nearly free, so it carries precision: an operand
+// per clock; 48 at N = 64 by that count), so 128 tokens x 16 heads cost 36 + 16 MMAs, 1,700 of the
+// about 3,300 clocks of their HBM time. N is nearly free, so it carries precision: an operand
 // that is not 8 bits already enters as a pair of e4m3 values side by side on N,
 // x = hi + lo / 16, about as precise as bf16 (8 significant bits) for x in [2^-6, 448]:
 //   scores  S^T[t][hi 16 | lo 16] = C[t][:] . Q[hi | lo]   (latent and rotary apart: their scales differ)
@@ -30,8 +30,7 @@
 // significant bits down to P' = 2^-20, 2^-24 of a typical largest one, fewer below, none
 // below 2^-28. The wider N costs an output MMA 8 clocks on 40, and shared memory and tensor
 // memory have room for one P and one output instead of two of each (256 x 4096: K2 106.3 us, 104.2
-// without).
-// Sums, scores and the output are fp32.
+// without). Sums, scores and the output are fp32.
 //
 // Pages (the plan's units) are TMA'd into a ring of five; a tile is up to two pages of a request. The
 // scores are M = 64 MMAs per page, so that a page needs no neighbour in the ring and its scores start

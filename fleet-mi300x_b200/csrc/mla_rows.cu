@@ -76,9 +76,9 @@ __global__ void __launch_bounds__(kRowsThreads) k_rows_to_pages(const MlaRowsToP
 // magnitudes meet in shared memory, then the rows are rounded and stored. A first block
 // that holds earlier rows of the request keeps the larger of the old and new scales and
 // holds those rows anew. 1,152 B read and 576 B written per row: 41 us for 131,072 rows,
-// 5.5 TB/s of the copy's 6.45. What keeps it from more is instruction issue (ncu: the SMs
-// 76 % busy at 46 us), so values stay packed bf16 pairs until the conversion and indexes are
-// 32-bit. Loading the next block ahead in persistent CTAs (64 us), or two blocks per CTA
+// 5.5 TB/s of the copy's 6.45. What keeps it from more is instruction issue (ncu: 238 warp
+// instructions per row, the SMs 69 % busy), so values stay packed bf16 pairs until the conversion and
+// indexes are 32-bit (before: 280, 76 %, 46 us). Loading the next block ahead in persistent CTAs (64 us), or two blocks per CTA
 // (51 us), was slower.
 //
 // Which block: request b owns the slots row_start[b] / 16 + 2 b .. row_start[b + 1] / 16
