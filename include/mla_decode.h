@@ -36,6 +36,10 @@
  * reference's in-place `cache[pos] = ...`, reference_decode.py:236-237) and
  * attends over rows 0..seq_lens[b] inclusive. It does not advance seq_lens;
  * the caller does, exactly as the reference's caller advances `pos`.
+ *
+ * The first kernel of a step may start while the kernel in front of it on the stream ends. Activations,
+ * seq_lens, rope_pos, the block table and the cache may be written by that kernel. Weights and RoPE tables are
+ * read ahead: a kernel that writes them may not be the one right in front of a step.
  */
 #ifndef MLA_DECODE_H_
 #define MLA_DECODE_H_
